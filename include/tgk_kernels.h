@@ -200,6 +200,53 @@ TGK_API int tgk_layernorm_bwd_rows(hipStream_t stream, int rows, int D, const ui
 TGK_API int tgk_layernorm_bwd_fold(hipStream_t stream, int rows, int D, int count, const void *partials,
                                    size_t job_stride_bytes, const void *targets, int accumulate);
 
+/* ---- RMS norm with the residual's addition (normalize and norm_backward, cuda/ops.cuh:57-80, at any width), outputs in
+ * bfloat16 and in 8 bits.  8-bit values are OCP e4m3 codes (uint8_t); every 128 columns of a row share a scale:
+ *   scale = max(max |v| / 448, 2^-100), code = RN_e4m3(v / scale), a value stands for code * scale.
+ * Scales lie [ceil(columns / 128)][ld_scales], ld_scales >= rows: those of a group of columns side by side, as tgk_gemm_q8 reads
+ * them.  A NaN has NaN's code and no part in the scale; with an infinity the scale is infinite and the group stands for NaN. ---- */
+
+/* h = RN_bf16(x + residual) into `sum` (may be x or residual itself); residual NULL: h = x, `sum` is not used.
+ * v = h * gamma / sqrt(mean(h^2) + eps) in fp32: RN_bf16(v) into y and / or codes into q and scales into `scales`; what is NULL is left out.
+ * x, residual, sum, y, q are [rows][D], D a multiple of 8, at most 8192; 16-byte aligned, q 8-byte. */
+TGK_API int tgk_rmsnorm_fwd(hipStream_t stream, int rows, int D, const uint16_t *x, const uint16_t *residual, const uint16_t *gamma_hi,
+                            const uint16_t *gamma_lo, uint16_t *sum, uint16_t *y, uint8_t *q, float *scales, int ld_scales, float eps);
+/* x is what was normalised (the forward's sum).  dx = RN(residual + dv), dv the gradient through the norm in fp32, or RN(dv) where
+ * residual is NULL; residual may be dx itself.  dgamma (=|+=) in fp32 in a fixed order.
+ * workspace: tgk_rmsnorm_bwd_workspace(rows, D) bytes, 16-byte aligned. */
+TGK_API int tgk_rmsnorm_bwd(hipStream_t stream, int rows, int D, const uint16_t *x, const uint16_t *dy, const uint16_t *gamma_hi,
+                            const uint16_t *gamma_lo, const uint16_t *residual, uint16_t *dx, float *dgamma, float eps, int accumulate,
+                            void *workspace, size_t workspace_bytes);
+TGK_API size_t tgk_rmsnorm_bwd_workspace(int rows, int D);
+
+/* bf16 rows [rows][ldx] into codes [rows][ldq] and scales as above.  columns and both leading dimensions multiples of 8. */
+TGK_API int tgk_quantize_rows(hipStream_t stream, int rows, int columns, const uint16_t *x, int ldx, uint8_t *q, int ldq, float *scales,
+                              int ld_scales);
+/* A weight: one scale for each tile of 128 x 128, scales [ceil(rows / 128)][ld_scales], ld_scales >= ceil(columns / 128). */
+TGK_API int tgk_quantize_tiles(hipStream_t stream, int rows, int columns, const uint16_t *w, int ldw, uint8_t *q, int ldq, float *scales,
+                               int ld_scales);
+
+/* The linear layer on such operands, beside tgk_gemm_fwd:
+ *   Y[m][n] = RN_bf16( sum_b x_scales[b][m] * w_scales[n / 128][b] * (sum over k in block b of X[m][k] W[n][k]) (+ residual[m][n]) )
+ * products and sums in fp32, rounded once.  Any M; N a multiple of 8, K of 16; ldx and ldw multiples of 16, ldy and ldr of 8; scales
+ * 4-byte, everything else 16-byte aligned.  The residual may be Y itself. */
+TGK_API int tgk_gemm_q8(hipStream_t stream, int M, int N, int K, const uint8_t *X, int ldx, const float *x_scales, int ldxs, const uint8_t *W,
+                        int ldw, const float *w_scales, int ldws, uint16_t *Y, int ldy, const uint16_t *residual, int ldr);
+
+/* ---- Gated feed-forward block (swiglu_activation and swiglu_backward, cuda/ops.cuh:120-144, at any width, with the projections).
+ * W[2F][D] holds the gate's rows and below them the up projection's (model.h:27-31).
+ *   [G U] = X W^T,  H = RN_bf16(act(G) U) from the fp32 sums;  GU[M][2F] = RN_bf16 of both, for the backward pass (NULL: not written)
+ * Any M, F and D multiples of 8; pointers 16-byte aligned, leading dimensions multiples of 8. ---- */
+enum { TGK_GATE_SILU = 0, TGK_GATE_GELU = 1 /* exact erf */ };
+TGK_API int tgk_gated_fwd(hipStream_t stream, int M, int F, int D, const uint16_t *X, int ldx, const uint16_t *W, int ldw, uint16_t *H, int ldh,
+                          uint16_t *GU, int ldgu, int activation);
+/* Backward from dY, the gradient of the block's output Y = H Wd^T (Wd[D][F], tgk_gemm_fwd), with the transposed copies of the
+ * weights (tgk_transpose_batch), Wdt[F][D] and Wt[D][2F]:
+ *   dH = dY Wd (not written),  dGU = [RN(dH U act'(G))  RN(dH act(G))],  dX = RN(dGU W); dX NULL: not computed, Wt not read.
+ * dGU may be GU itself.  The weights' gradients are tgk_gemm_wgrad products: dW[2F][D] = dGU^T X and dWd = dY^T H. */
+TGK_API int tgk_gated_bwd(hipStream_t stream, int M, int F, int D, const uint16_t *dY, int lddy, const uint16_t *Wdt, int ldwdt, const uint16_t *GU,
+                          int ldgu, uint16_t *dGU, int lddgu, const uint16_t *Wt, int ldwt, uint16_t *dX, int lddx, int activation);
+
 /* Softmax cross-entropy over 256 byte classes on bf16 logits [rows][256] (cuda/model.cuh:33-58):
  * loss[t] = logsumexp - logit[y[t]]; logits_f32 (optional) receives the logits as fp32;
  * write_grad != 0 overwrites the logits with RN_bf16((softmax - onehot) * inv_count). */

@@ -47,6 +47,14 @@ KERNEL_ABI = {
     "tgk_layernorm_bwd_workspace": (sz, [i32, i32]),
     "tgk_layernorm_bwd_rows": (i32, [vp, i32, i32, vp, vp, vp, vp, vp, vp, f32, vp, sz]),
     "tgk_layernorm_bwd_fold": (i32, [vp, i32, i32, i32, vp, sz, vp, i32]),
+    "tgk_rmsnorm_fwd": (i32, [vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, i32, f32]),
+    "tgk_rmsnorm_bwd": (i32, [vp, i32, i32, vp, vp, vp, vp, vp, vp, vp, f32, i32, vp, sz]),
+    "tgk_rmsnorm_bwd_workspace": (sz, [i32, i32]),
+    "tgk_quantize_rows": (i32, [vp, i32, i32, vp, i32, vp, i32, vp, i32]),
+    "tgk_quantize_tiles": (i32, [vp, i32, i32, vp, i32, vp, i32, vp, i32]),
+    "tgk_gemm_q8": (i32, [vp, i32, i32, i32, vp, i32, vp, i32, vp, i32, vp, i32, vp, i32, vp, i32]),
+    "tgk_gated_fwd": (i32, [vp, i32, i32, i32, vp, i32, vp, i32, vp, i32, vp, i32, i32]),
+    "tgk_gated_bwd": (i32, [vp, i32, i32, i32, vp, i32, vp, i32, vp, i32, vp, i32, vp, i32, vp, i32, i32]),
     "tgk_cross_entropy": (i32, [vp, i32, i32, vp, vp, vp, vp, f32, i32]),
     "tgk_sumsq_partials": (i32, [vp, vp, sz, vp, i32]),
     "tgk_sumsq_segments": (i32, [vp, vp, vp, i32, vp]),

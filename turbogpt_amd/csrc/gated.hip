@@ -1,0 +1,173 @@
+// The gated feed-forward block, H = act(X Wg^T) * (X Wu^T), and its backward pass.  W = [Wg; Wu] is packed [2F][D], the layout
+// of the width-16 network's gate and up projections (model.h:27-31; swiglu_activation and swiglu_backward, cuda/ops.cuh:120-144).
+//
+// Forward: one product whose tiles hold 32 gate and the same 32 up columns per wave, so that a lane has both pre-activations
+// of an output and nothing but H (and, for training, the pre-activations) is written.
+// Backward, from the gradient of the block's output Y = H Wd^T: dH = dY Wd is a product whose epilogue reads the saved
+// pre-activations and writes dG = dH u act'(g) and dU = dH act(g); dH itself never reaches memory.  dX = [dG dU] W is a plain
+// product over 2F.  The weights' gradients are dW = [dG dU]^T X and dWd = dY^T H: tgk_gemm_wgrad.
+#include "product_tile.h"
+#include "../../include/tgk_kernels.h"
+
+namespace {
+using namespace product;
+
+// SiLU and its derivative from one exponential: s = 1 / (1 + e^-g), g s and s (1 + g (1 - s)).  A reciprocal of an
+// infinite 1 + e^-g is 0, so the far negative side gives -0 and not NaN, but g = -inf gives NaN as the formula does.
+struct Gate {
+    float act, slope;
+};
+template <int ACT> TG_DEVICE float act_f(float g) {
+    if constexpr (ACT == TGK_GATE_SILU)
+        return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g));
+    else
+        return gelu_f(g);
+}
+template <int ACT> TG_DEVICE Gate gate_f(float g) {
+    if constexpr (ACT == TGK_GATE_SILU) {
+        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g));
+        return {g * s, s * fmaf(g, 1.0f - s, 1.0f)};
+    } else {
+        return {gelu_f(g), gelu_grad_f(g)};
+    }
+}
+
+template <int ACT, bool KEEP> struct GatedForward {
+    bf16_t *h, *gu;
+    int ld_h, ld_gu;
+    // The activation and the product are taken of the 32-bit sums and rounded once; what is kept for the backward pass is
+    // rounded by itself.
+    template <class T> TG_DEVICE void finish(const Shape &s, const f32x4 (&acc)[T::FM][T::FN], unsigned char *staging, int m_base, int n_base, int lane) const {
+        const int r = lane >> 2, q = lane & 3, f = n_base + q * 8;
+#pragma unroll
+        for (int i = 0; i < T::FM; ++i) {
+            stage_results<T>(acc[i], staging, lane);
+            float g[8], u[8], v[8];
+            staged8(staging, r, q, g);
+            staged8(staging, r, 4 + q, u);
+            const int m = m_base + i * 16 + r;
+            if (m < s.M && f < s.N) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    v[e] = act_f<ACT>(g[e]) * u[e];
+                *reinterpret_cast<u32x4 *>(h + size_t(m) * ld_h + f) = pack8(v);
+                if constexpr (KEEP) {
+                    *reinterpret_cast<u32x4 *>(gu + size_t(m) * ld_gu + f) = pack8(g);
+                    *reinterpret_cast<u32x4 *>(gu + size_t(m) * ld_gu + s.N + f) = pack8(u);
+                }
+            }
+        }
+    }
+};
+
+template <int ACT> struct GatedBackward {
+    const bf16_t *gu; // may be dgu: every lane reads its values before it writes them
+    bf16_t *dgu;
+    int ld_gu, ld_dgu;
+    template <class T> TG_DEVICE void finish(const Shape &s, const f32x4 (&acc)[T::FM][T::FN], unsigned char *staging, int m_base, int n_base, int lane) const {
+#pragma unroll
+        for (int i = 0; i < T::FM; ++i) {
+            stage_results<T>(acc[i], staging, lane);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int r = (lane >> 3) + half * 8, q = lane & 7, m = m_base + i * 16 + r, f = n_base + q * 8;
+                float dh[8], g[8], u[8];
+                staged8(staging, r, q, dh);
+                if (m < s.M && f < s.N) {
+                    unpack8(*reinterpret_cast<const u32x4 *>(gu + size_t(m) * ld_gu + f), g);
+                    unpack8(*reinterpret_cast<const u32x4 *>(gu + size_t(m) * ld_gu + s.N + f), u);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const Gate gate = gate_f<ACT>(g[e]);
+                        g[e] = dh[e] * u[e] * gate.slope;
+                        u[e] = dh[e] * gate.act;
+                    }
+                    *reinterpret_cast<u32x4 *>(dgu + size_t(m) * ld_dgu + f) = pack8(g);
+                    *reinterpret_cast<u32x4 *>(dgu + size_t(m) * ld_dgu + s.N + f) = pack8(u);
+                }
+            }
+        }
+    }
+};
+
+struct Plain {
+    bf16_t *out;
+    int ld_out;
+    template <class T> TG_DEVICE void finish(const Shape &s, const f32x4 (&acc)[T::FM][T::FN], unsigned char *staging, int m_base, int n_base, int lane) const {
+#pragma unroll
+        for (int i = 0; i < T::FM; ++i) {
+            stage_results<T>(acc[i], staging, lane);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int r = (lane >> 3) + half * 8, q = lane & 7, m = m_base + i * 16 + r, n = n_base + q * 8;
+                float v[8];
+                staged8(staging, r, q, v);
+                if (m < s.M && n < s.N)
+                    *reinterpret_cast<u32x4 *>(out + size_t(m) * ld_out + n) = pack8(v);
+            }
+        }
+    }
+};
+
+template <bool GATED, class Epilogue> void product_bf16(hipStream_t stream, int M, int N, int K, const bf16_t *a, int lda, const bf16_t *b, int ldb, const Epilogue &epilogue) {
+    Shape s{};
+    s.a = reinterpret_cast<const unsigned char *>(a), s.b = reinterpret_cast<const unsigned char *>(b);
+    s.lda = int64_t(lda) * 2, s.ldb = int64_t(ldb) * 2;
+    s.M = M, s.N = N, s.k_bytes = K * 2;
+    launch_product<false, GATED>(stream, s, epilogue);
+}
+
+void operand(const void *p, int ld, int columns, const char *what) {
+    if (!p || reinterpret_cast<uintptr_t>(p) & 15 || ld < columns || ld % 8 || ld > MOST_LD)
+        throw std::invalid_argument(std::string(what) + ": needs a 16-byte aligned pointer and a leading dimension that is a multiple of 8, at least the columns and at most 2^21");
+}
+void block_shape(int M, int F, int D, int activation, const char *where) {
+    if (M < 1 || F < 8 || D < 8 || F % 8 || D % 8 || F > MOST_LD / 2 || D > MOST_LD)
+        throw std::invalid_argument(std::string(where) + ": M at least 1, F and D multiples of 8 (F at most 2^20, D at most 2^21)");
+    if (activation != TGK_GATE_SILU && activation != TGK_GATE_GELU)
+        throw std::invalid_argument(std::string(where) + ": activation is TGK_GATE_SILU or TGK_GATE_GELU");
+}
+template <class F> void by_activation(int activation, F &&f) {
+    if (activation == TGK_GATE_SILU)
+        f(std::integral_constant<int, TGK_GATE_SILU>{});
+    else
+        f(std::integral_constant<int, TGK_GATE_GELU>{});
+}
+} // namespace
+
+extern "C" int tgk_gated_fwd(hipStream_t stream, int M, int F, int D, const uint16_t *X, int ldx, const uint16_t *W, int ldw, uint16_t *H, int ldh,
+                             uint16_t *GU, int ldgu, int activation) {
+    return guarded([&] {
+        block_shape(M, F, D, activation, "gated_fwd");
+        operand(X, ldx, D, "gated_fwd: X");
+        operand(W, ldw, D, "gated_fwd: W");
+        operand(H, ldh, F, "gated_fwd: H");
+        if (GU)
+            operand(GU, ldgu, 2 * F, "gated_fwd: GU");
+        by_activation(activation, [&](auto act) {
+            if (GU)
+                product_bf16<true>(stream, M, F, D, X, ldx, W, ldw, GatedForward<act(), true>{H, GU, ldh, ldgu});
+            else
+                product_bf16<true>(stream, M, F, D, X, ldx, W, ldw, GatedForward<act(), false>{H, nullptr, ldh, 0});
+        });
+    });
+}
+
+extern "C" int tgk_gated_bwd(hipStream_t stream, int M, int F, int D, const uint16_t *dY, int lddy, const uint16_t *Wdt, int ldwdt, const uint16_t *GU, int ldgu,
+                             uint16_t *dGU, int lddgu, const uint16_t *Wt, int ldwt, uint16_t *dX, int lddx, int activation) {
+    return guarded([&] {
+        block_shape(M, F, D, activation, "gated_bwd");
+        operand(dY, lddy, D, "gated_bwd: dY");
+        operand(Wdt, ldwdt, D, "gated_bwd: Wdt");
+        operand(GU, ldgu, 2 * F, "gated_bwd: GU");
+        operand(dGU, lddgu, 2 * F, "gated_bwd: dGU");
+        require(GU != dGU || ldgu == lddgu, "gated_bwd: in place, GU and dGU have the same leading dimension");
+        if (dX) {
+            operand(Wt, ldwt, 2 * F, "gated_bwd: Wt");
+            operand(dX, lddx, D, "gated_bwd: dX");
+        }
+        by_activation(activation, [&](auto act) { product_bf16<false>(stream, M, F, D, dY, lddy, Wdt, ldwdt, GatedBackward<act()>{GU, dGU, ldgu, lddgu}); });
+        if (dX)
+            product_bf16<false>(stream, M, D, 2 * F, dGU, lddgu, Wt, ldwt, Plain{dX, lddx});
+    });
+}

@@ -1,0 +1,281 @@
+// Products C[m][n] = sum_k A(m,k) B(n,k) of any number of rows and columns, for the operators whose results leave in a
+// form of their own (gated.hip, gemm_q8.hip).  Both operands are k-contiguous; a row's K is `k_bytes` long, a multiple of 16.
+//
+// A stage is 128 bytes of k of every row of a tile, 64 values in bfloat16 and 128 in e4m3, so that every copy asks for whole
+// lines and one body serves both.  Copies go straight to LDS (async_copy16).  Row r's 16-byte chunk c lies at chunk c ^ (r & 7).
+// A lane's fragment of rows r0 + lane % 16 is the chunk pair lane / 16 and lane / 16 + 4: which k a chunk holds does not
+// matter as long as both operands are read alike.
+//
+// Rows outside the operands are read as the last row inside (their results are not stored), so no address leaves the
+// operands; chunks behind the end of k are read from the stage's first chunk and overwritten with zeros in both operands
+// before the stage is published, as what lies behind a row's end may be anything, NaN included.
+#pragma once
+#include "common.h"
+#include <atomic>
+#include <type_traits>
+
+namespace product {
+
+constexpr int STAGE = 128; // bytes of k
+
+struct Shape {
+    const unsigned char *a, *b;
+    int64_t lda, ldb;    // bytes from row to row
+    int M, N;            // rows of a; rows of b, or (gated) half of them: columns of the result
+    int k_bytes, stages; // stages = ceil(k_bytes / STAGE)
+    int tiles_m, tiles_n, tiles;
+    const float *a_scales, *b_scales; // of 8-bit operands: [stage][ld_a_scales] by row, [row / 128][ld_b_scales] by stage
+    int ld_a_scales, ld_b_scales;
+};
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// WM x WN waves of (BM / WM) x 64 outputs.  AR: slots of A's ring (2 or 3; B's has 2), a stage of A is requested AR - 1
+// stages ahead.  GATED: B's rows are of two matrices on top of each other, N rows each; every wave's 64 are 32 of the upper
+// and the same 32 of the lower, and a tile has BN / 2 columns of the result.
+template <bool E4M3_, bool GATED_, int BM_, int BN_, int WM_, int WN_, int AR_> struct Tile {
+    static constexpr bool E4M3 = E4M3_, GATED = GATED_;
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, AR = AR_, WAVES = WM * WN, THREADS = WAVES * 64;
+    static constexpr int FM = BM / WM / 16, FN = 4, COLUMNS = GATED ? BN / 2 : BN;
+    static constexpr int A_COPIES = BM / 8 / WAVES, B_COPIES = BN / 8 / WAVES, SCALE_COPIES = E4M3 ? 1 : 0;
+    static constexpr int A_BYTES = BM * STAGE, B_BYTES = BN * STAGE;
+    static constexpr int SCALE_BYTES = E4M3 ? BM * 4 + 256 : 0; // a slot: the rows' scales, then 64 floats of the columns'
+    static constexpr int STAGING_BYTES = 4096;                  // a wave's 16 x 64 results
+    static constexpr int B_AT = AR * A_BYTES, SCALES_AT = B_AT + 2 * B_BYTES, LDS_BYTES = SCALES_AT + AR * SCALE_BYTES;
+    static_assert(BN / WN == 64 && BN <= 256 && BM / 64 <= WAVES / (E4M3 ? 2 : 1) && B_BYTES >= WAVES * STAGING_BYTES, "tile");
+};
+
+// the wave's 16 x 64 results of fragment row i, left in its staging buffer: 16-byte chunk c (4 columns) of row r at c ^ r
+template <class T> TG_DEVICE void stage_results(const f32x4 (&row)[T::FN], unsigned char *staging, int lane) {
+    const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < T::FN; ++j)
+        *reinterpret_cast<f32x4 *>(staging + r * 256 + (((j * 4 + g) ^ r) << 4)) = row[j];
+}
+// columns 8 q .. 8 q + 7 of row r of them
+TG_DEVICE void staged8(const unsigned char *staging, int r, int q, float (&v)[8]) {
+    const f32x4 lo = *reinterpret_cast<const f32x4 *>(staging + r * 256 + (((2 * q) ^ r) << 4));
+    const f32x4 hi = *reinterpret_cast<const f32x4 *>(staging + r * 256 + (((2 * q + 1) ^ r) << 4));
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        v[e] = lo[e], v[4 + e] = hi[e];
+}
+TG_DEVICE u32x4 pack8(const float (&v)[8]) {
+    return u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+}
+TG_DEVICE void unpack8(const u32x4 &p, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        v[2 * e] = bf16_lo(p[e]), v[2 * e + 1] = bf16_hi(p[e]);
+}
+
+// One operand's place in the block's list of stages, and the lane's addresses there.
+template <class T, bool IS_A> struct Producer {
+    static constexpr int COPIES = IS_A ? T::A_COPIES : T::B_COPIES;
+    int tile, stage, slot;
+    const unsigned char *base; // the tile's first row
+    uint32_t offset[COPIES];   // of the lane's row and chunk
+    int64_t low_rows;          // bytes from the upper matrix's rows to the lower one's
+    int m0;
+
+    TG_DEVICE void start(const Shape &s, int first_tile, int wave, int lane) {
+        tile = first_tile, stage = 0, slot = 0;
+        low_rows = s.ldb * s.N;
+        enter(s, wave, lane);
+    }
+    TG_DEVICE void enter(const Shape &s, int wave, int lane) {
+        const int tn = tile % s.tiles_n, tm = tile / s.tiles_n;
+        const int first = IS_A ? tm * T::BM : tn * T::COLUMNS, rows = IS_A ? s.M : s.N;
+        const int64_t ld = IS_A ? s.lda : s.ldb;
+        base = (IS_A ? s.a : s.b) + first * ld;
+        m0 = tm * T::BM;
+        const int chunk = (lane & 7) ^ (lane >> 3);
+#pragma unroll
+        for (int j = 0; j < COPIES; ++j) {
+            const int group = j * T::WAVES + wave; // of 8 rows
+            int row = group * 8 + (lane >> 3);
+            if (T::GATED && !IS_A)
+                row = (group >> 3) * 32 + (group & 3) * 8 + (lane >> 3);
+            row = row < rows - first ? row : rows - first - 1;
+            offset[j] = uint32_t(row) * uint32_t(ld) + chunk * 16;
+        }
+    }
+    // chunks of this stage that the operands have
+    TG_DEVICE int chunks(const Shape &s) const { return (s.k_bytes - stage * STAGE + 15) >> 4; }
+    TG_DEVICE void copy(const Shape &s, uint32_t ring, int wave, int lane) const {
+        const int chunk = (lane & 7) ^ (lane >> 3), have = chunks(s);
+        const uint32_t back = chunk < have ? 0u : uint32_t(chunk * 16); // behind the end of k: the stage's first chunk
+        const uint32_t to = ring + slot * (IS_A ? T::A_BYTES : T::B_BYTES);
+#pragma unroll
+        for (int j = 0; j < COPIES; ++j) {
+            const int group = j * T::WAVES + wave;
+            const unsigned char *from = base + stage * STAGE;
+            if (T::GATED && !IS_A && (group & 4))
+                from += low_rows;
+            async_copy16(to + group * 1024, from, offset[j] - back);
+        }
+    }
+    // A's rows' scales by one half of the waves, the columns' by the other: 64 floats each
+    TG_DEVICE void copy_scales(const Shape &s, uint32_t ring, int wave, int lane) const {
+        const uint32_t to = ring + slot * T::SCALE_BYTES;
+        if (wave < T::WAVES / 2) {
+            const int part = wave % (T::BM / 64), m = m0 + part * 64 + lane;
+            async_copy4(to + part * 256, s.a_scales + int64_t(stage) * s.ld_a_scales + (m < s.M ? m : s.M - 1));
+        } else {
+            const int first = tile % s.tiles_n * (T::BN / 128), last = (s.N - 1) / 128;
+            const int n = first + (lane & 1) < last ? first + (lane & 1) : last;
+            async_copy4(to + T::BM * 4, s.b_scales + int64_t(n) * s.ld_b_scales + stage);
+        }
+    }
+    // after the wave's copies of a stage with too few chunks have landed, where they lie in `slot_at`
+    TG_DEVICE static void clear_tail(uint32_t slot_at, int have, int wave, int lane) {
+        const int chunk = (lane & 7) ^ (lane >> 3);
+        if (chunk < have)
+            return;
+#pragma unroll
+        for (int j = 0; j < COPIES; ++j)
+            *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(slot_at + (j * T::WAVES + wave) * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
+    }
+    TG_DEVICE void advance(const Shape &s, int step, int wave, int lane) {
+        slot = slot + 1 == (IS_A ? T::AR : 2) ? 0 : slot + 1;
+        if (stage + 1 < s.stages)
+            ++stage;
+        else if (tile + step < s.tiles) // otherwise the last stage again: the number of copies in flight stays the same
+            tile += step, stage = 0, enter(s, wave, lane);
+    }
+};
+
+// Tiles in the order in which a block meets them: a block's neighbours in its XCD (blocks 8 apart) take neighbouring tiles,
+// which share rows of a and b in that XCD's L2.
+TG_DEVICE int first_tile(int block, int grid) {
+    const int each = grid >> 3, rest = grid & 7, xcd = block & 7;
+    return xcd * each + (xcd < rest ? xcd : rest) + (block >> 3);
+}
+
+template <class T, class Epilogue> __global__ __launch_bounds__(T::THREADS, T::LDS_BYTES > 81920 ? T::WAVES / 4 : T::WAVES / 2)
+void tile_kernel(Shape s, Epilogue epilogue) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / T::WN, wn = wave % T::WN, step = gridDim.x;
+    const uint32_t at = lds_address(lds);
+    Producer<T, true> pa;
+    Producer<T, false> pb;
+    pa.start(s, first_tile(blockIdx.x, step), wave, lane);
+    pb.start(s, first_tile(blockIdx.x, step), wave, lane);
+    const auto request_a = [&] {
+        if constexpr (T::E4M3)
+            pa.copy_scales(s, at + T::SCALES_AT, wave, lane);
+        pa.copy(s, at, wave, lane);
+        pa.advance(s, step, wave, lane);
+    };
+    const auto request_b = [&] {
+        pb.copy(s, at + T::B_AT, wave, lane);
+        pb.advance(s, step, wave, lane);
+    };
+    request_b();
+    request_a();
+    if constexpr (T::AR == 3)
+        request_a();
+    const int tail = (s.k_bytes % STAGE + 15) >> 4; // chunks of the last stage, 0: all
+    const auto publish = [&](bool is_tail, int slot_a, int slot_b) {
+        wait_vmcnt<T::AR == 3 ? T::A_COPIES + T::SCALE_COPIES : 0>();
+        if (is_tail) {
+            Producer<T, true>::clear_tail(at + slot_a * T::A_BYTES, tail, wave, lane);
+            Producer<T, false>::clear_tail(at + T::B_AT + slot_b * T::B_BYTES, tail, wave, lane);
+            wait_lgkmcnt0();
+        }
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    publish(tail && s.stages == 1, 0, 0);
+    int slot_a = 0, slot_b = 0;
+    const uint32_t lane_at = (lane & 15) * STAGE + (((lane >> 4) ^ (lane & 7)) << 4);
+    const auto chunk_at = [](uint32_t address) { return *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)address; };
+    for (int tile = first_tile(blockIdx.x, step); tile < s.tiles; tile += step) {
+        f32x4 acc[T::FM][T::FN];
+#pragma unroll
+        for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+            for (int j = 0; j < T::FN; ++j)
+                acc[i][j] = f32x4{0, 0, 0, 0};
+        for (int stage = 0; stage < s.stages; ++stage) {
+            request_b();
+            request_a();
+            const uint32_t a_at = at + slot_a * T::A_BYTES + wm * (T::FM * 16 * STAGE) + lane_at;
+            const uint32_t b_at = at + T::B_AT + slot_b * T::B_BYTES + wn * (T::FN * 16 * STAGE) + lane_at;
+            u32x4 b[T::FN][2];
+#pragma unroll
+            for (int j = 0; j < T::FN; ++j) {
+                b[j][0] = chunk_at(b_at + j * 2048);
+                b[j][1] = chunk_at((b_at + j * 2048) ^ 64);
+            }
+            if constexpr (T::E4M3) {
+                const unsigned char *scales = lds + T::SCALES_AT + slot_a * T::SCALE_BYTES;
+                const float column = *reinterpret_cast<const float *>(scales + T::BM * 4 + ((wn * 64) >> 7) * 4);
+#pragma unroll
+                for (int i = 0; i < T::FM; ++i) {
+                    const u32x4 low = chunk_at(a_at + i * 2048), high = chunk_at((a_at + i * 2048) ^ 64);
+                    const float scale = column * *reinterpret_cast<const float *>(scales + (wm * T::FM * 16 + i * 16 + (lane & 15)) * 4);
+                    const i32x8 a = __builtin_bit_cast(i32x8, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int j = 0; j < T::FN; ++j) {
+                        const i32x8 w = __builtin_bit_cast(i32x8, __builtin_shufflevector(b[j][0], b[j][1], 0, 1, 2, 3, 4, 5, 6, 7));
+                        const f32x4 part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, f32x4{0, 0, 0, 0}, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            acc[i][j][e] = fmaf(part[e], scale, acc[i][j][e]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < T::FM; ++i) {
+                    const bf16x8 low = __builtin_bit_cast(bf16x8, chunk_at(a_at + i * 2048));
+                    const bf16x8 high = __builtin_bit_cast(bf16x8, chunk_at((a_at + i * 2048) ^ 64));
+#pragma unroll
+                    for (int j = 0; j < T::FN; ++j) {
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b[j][0]), low, acc[i][j], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b[j][1]), high, acc[i][j], 0, 0, 0);
+                    }
+                }
+            }
+            const int read_b = slot_b;
+            slot_a = slot_a + 1 == T::AR ? 0 : slot_a + 1;
+            slot_b ^= 1;
+            const int next = stage + 1 < s.stages ? stage + 1 : 0; // of this tile or the block's next
+            publish(tail && next + 1 == s.stages, slot_a, slot_b);
+            if (stage + 1 == s.stages) {
+                // every wave has left B's slot that was read, and no copy into it has been requested yet
+                epilogue.template finish<T>(s, acc, lds + T::B_AT + read_b * T::B_BYTES + wave * T::STAGING_BYTES, tile / s.tiles_n * T::BM + wm * T::FM * 16,
+                                            tile % s.tiles_n * T::COLUMNS + wn * (T::COLUMNS / T::WN), lane);
+                wait_lgkmcnt0();
+                __builtin_amdgcn_s_barrier(); // the next stage's copies go into that slot
+                asm volatile("" ::: "memory");
+            }
+        }
+    }
+    wait_vmcnt<0>(); // no copy may land after the block's LDS has gone to another
+}
+
+// A lane's offset into a tile is 32 bits wide: 256 rows of at most 2^22 bytes.
+constexpr int MOST_LD = 1 << 21; // elements of 16 bits
+
+template <class T, class Epilogue> void launch_tiles(hipStream_t stream, Shape s, const Epilogue &epilogue) {
+    s.tiles_m = (s.M + T::BM - 1) / T::BM, s.tiles_n = (s.N + T::COLUMNS - 1) / T::COLUMNS;
+    require(int64_t(s.tiles_m) * s.tiles_n < (int64_t(1) << 30), "product: too many tiles");
+    s.tiles = s.tiles_m * s.tiles_n, s.stages = (s.k_bytes + STAGE - 1) / STAGE;
+    const int most = T::LDS_BYTES > 81920 ? 256 : 512;
+    static std::atomic<uint64_t> configured; // devices whose LDS opt-in for this kernel has been made
+    int device = 0;
+    check_hip(hipGetDevice(&device), "product: ");
+    if (!(configured.load(std::memory_order_acquire) >> (device & 63) & 1)) {
+        check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(tile_kernel<T, Epilogue>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS_BYTES), "product LDS size: ");
+        configured.fetch_or(uint64_t(1) << (device & 63), std::memory_order_release);
+    }
+    hipLaunchKernelGGL((tile_kernel<T, Epilogue>), dim3(s.tiles < most ? s.tiles : most), dim3(T::THREADS), T::LDS_BYTES, stream, s, epilogue);
+    check_hip(hipGetLastError(), "product launch: ");
+}
+template <bool E4M3, bool GATED, class Epilogue> void launch_product(hipStream_t stream, const Shape &s, const Epilogue &epilogue) {
+    launch_tiles<Tile<E4M3, GATED, 128, 128, 2, 2, 2>>(stream, s, epilogue);
+}
+
+} // namespace product
