@@ -41,6 +41,7 @@ template <int ACT, bool KEEP> struct GatedForward {
         const int r = lane >> 2, q = lane & 3, f = n_base + q * 8;
 #pragma unroll
         for (int i = 0; i < T::FM; ++i) {
+            __builtin_amdgcn_sched_barrier(0); // one fragment row at a time: hoisted loads would not leave the sums their registers
             stage_results<T>(acc[i], staging, lane);
             float g[8], u[8], v[8];
             staged8(staging, r, q, g);
@@ -67,6 +68,7 @@ template <int ACT> struct GatedBackward {
     template <class T> TG_DEVICE void finish(const Shape &s, const f32x4 (&acc)[T::FM][T::FN], unsigned char *staging, int m_base, int n_base, int lane) const {
 #pragma unroll
         for (int i = 0; i < T::FM; ++i) {
+            __builtin_amdgcn_sched_barrier(0); // one fragment row at a time: hoisted loads would not leave the sums their registers
             stage_results<T>(acc[i], staging, lane);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -96,6 +98,7 @@ struct Plain {
     template <class T> TG_DEVICE void finish(const Shape &s, const f32x4 (&acc)[T::FM][T::FN], unsigned char *staging, int m_base, int n_base, int lane) const {
 #pragma unroll
         for (int i = 0; i < T::FM; ++i) {
+            __builtin_amdgcn_sched_barrier(0); // one fragment row at a time: hoisted loads would not leave the sums their registers
             stage_results<T>(acc[i], staging, lane);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {

@@ -16,6 +16,7 @@ template <bool ADD> struct Residual {
     template <class T> TG_DEVICE void finish(const Shape &s, const f32x4 (&acc)[T::FM][T::FN], unsigned char *staging, int m_base, int n_base, int lane) const {
 #pragma unroll
         for (int i = 0; i < T::FM; ++i) {
+            __builtin_amdgcn_sched_barrier(0); // one fragment row at a time: hoisted loads would not leave the sums their registers
             stage_results<T>(acc[i], staging, lane);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {

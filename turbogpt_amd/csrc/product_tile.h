@@ -33,8 +33,8 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 // WM x WN waves of (BM / WM) x 64 outputs.  AR: slots of A's ring (2 or 3; B's has 2), a stage of A is requested AR - 1
 // stages ahead.  GATED: B's rows are of two matrices on top of each other, N rows each; every wave's 64 are 32 of the upper
 // and the same 32 of the lower, and a tile has BN / 2 columns of the result.
-template <bool E4M3_, bool GATED_, int BM_, int BN_, int WM_, int WN_, int AR_> struct Tile {
-    static constexpr bool E4M3 = E4M3_, GATED = GATED_;
+template <bool E4M3_, bool GATED_, int BM_, int BN_, int WM_, int WN_, int AR_, bool PHASED_ = false> struct Tile {
+    static constexpr bool E4M3 = E4M3_, GATED = GATED_, PHASED = PHASED_;
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, AR = AR_, WAVES = WM * WN, THREADS = WAVES * 64;
     static constexpr int FM = BM / WM / 16, FN = 4, COLUMNS = GATED ? BN / 2 : BN;
     static constexpr int A_COPIES = BM / 8 / WAVES, B_COPIES = BN / 8 / WAVES, SCALE_COPIES = E4M3 ? 1 : 0;
@@ -69,6 +69,16 @@ TG_DEVICE void unpack8(const u32x4 &p, float (&v)[8]) {
         v[2 * e] = bf16_lo(p[e]), v[2 * e + 1] = bf16_hi(p[e]);
 }
 
+// Tiles are walked in bands of four rows of tiles, column by column: 32 neighbours, what an XCD works on at a time, are 4 x 8 tiles
+// and share 12 panels of the operands in its L2, where 32 in one row would share 33.
+constexpr int BAND = 4;
+TG_DEVICE void place(const Shape &s, int tile, int &tm, int &tn) {
+    const int per_band = BAND * s.tiles_n, band = tile / per_band, in = tile - band * per_band;
+    const int rows = s.tiles_m - band * BAND < BAND ? s.tiles_m - band * BAND : BAND;
+    tn = in / rows;
+    tm = band * BAND + in - tn * rows;
+}
+
 // One operand's place in the block's list of stages, and the lane's addresses there.
 template <class T, bool IS_A> struct Producer {
     static constexpr int COPIES = IS_A ? T::A_COPIES : T::B_COPIES;
@@ -76,7 +86,7 @@ template <class T, bool IS_A> struct Producer {
     const unsigned char *base; // the tile's first row
     uint32_t offset[COPIES];   // of the lane's row and chunk
     int64_t low_rows;          // bytes from the upper matrix's rows to the lower one's
-    int m0;
+    int m0, n0;                // the tile's first row; its column in tiles
 
     TG_DEVICE void start(const Shape &s, int first_tile, int wave, int lane) {
         tile = first_tile, stage = 0, slot = 0;
@@ -84,11 +94,12 @@ template <class T, bool IS_A> struct Producer {
         enter(s, wave, lane);
     }
     TG_DEVICE void enter(const Shape &s, int wave, int lane) {
-        const int tn = tile % s.tiles_n, tm = tile / s.tiles_n;
+        int tm, tn;
+        place(s, tile, tm, tn);
         const int first = IS_A ? tm * T::BM : tn * T::COLUMNS, rows = IS_A ? s.M : s.N;
         const int64_t ld = IS_A ? s.lda : s.ldb;
         base = (IS_A ? s.a : s.b) + first * ld;
-        m0 = tm * T::BM;
+        m0 = tm * T::BM, n0 = tn;
         const int chunk = (lane & 7) ^ (lane >> 3);
 #pragma unroll
         for (int j = 0; j < COPIES; ++j) {
@@ -122,7 +133,7 @@ template <class T, bool IS_A> struct Producer {
             const int part = wave % (T::BM / 64), m = m0 + part * 64 + lane;
             async_copy4(to + part * 256, s.a_scales + int64_t(stage) * s.ld_a_scales + (m < s.M ? m : s.M - 1));
         } else {
-            const int first = tile % s.tiles_n * (T::BN / 128), last = (s.N - 1) / 128;
+            const int first = n0 * (T::BN / 128), last = (s.N - 1) / 128;
             const int n = first + (lane & 1) < last ? first + (lane & 1) : last;
             async_copy4(to + T::BM * 4, s.b_scales + int64_t(n) * s.ld_b_scales + stage);
         }
@@ -144,6 +155,11 @@ template <class T, bool IS_A> struct Producer {
             tile += step, stage = 0, enter(s, wave, lane);
     }
 };
+
+// The value is there by now: products whose results are used phases later would otherwise be moved behind the barriers.
+TG_DEVICE void pin(f32x4 &v) {
+    asm volatile("" : "+v"(v));
+}
 
 // Tiles in the order in which a block meets them: a block's neighbours in its XCD (blocks 8 apart) take neighbouring tiles,
 // which share rows of a and b in that XCD's L2.
@@ -177,19 +193,33 @@ void tile_kernel(Shape s, Epilogue epilogue) {
     if constexpr (T::AR == 3)
         request_a();
     const int tail = (s.k_bytes % STAGE + 15) >> 4; // chunks of the last stage, 0: all
-    const auto publish = [&](bool is_tail, int slot_a, int slot_b) {
+    const auto landed = [&](bool is_tail, int slot_a, int slot_b) {
         wait_vmcnt<T::AR == 3 ? T::A_COPIES + T::SCALE_COPIES : 0>();
         if (is_tail) {
             Producer<T, true>::clear_tail(at + slot_a * T::A_BYTES, tail, wave, lane);
             Producer<T, false>::clear_tail(at + T::B_AT + slot_b * T::B_BYTES, tail, wave, lane);
             wait_lgkmcnt0();
         }
+    };
+    // behind it, what the wave has read from LDS may be overwritten
+    const auto turn = [] {
+        __builtin_amdgcn_sched_barrier(0);
+        wait_lgkmcnt0();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto publish = [&](bool is_tail, int slot_a, int slot_b) {
+        landed(is_tail, slot_a, slot_b);
+        turn();
     };
     publish(tail && s.stages == 1, 0, 0);
     int slot_a = 0, slot_b = 0;
     const uint32_t lane_at = (lane & 15) * STAGE + (((lane >> 4) ^ (lane & 7)) << 4);
+    const auto block_at = [](uint32_t address) { // both chunks of a lane
+        const u32x4 low = *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)address, high = *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)(address ^ 64);
+        return __builtin_bit_cast(i32x8, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
     const auto chunk_at = [](uint32_t address) { return *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)address; };
     for (int tile = first_tile(blockIdx.x, step); tile < s.tiles; tile += step) {
         f32x4 acc[T::FM][T::FN];
@@ -198,60 +228,156 @@ void tile_kernel(Shape s, Epilogue epilogue) {
 #pragma unroll
             for (int j = 0; j < T::FN; ++j)
                 acc[i][j] = f32x4{0, 0, 0, 0};
+        constexpr int PHASES = 4, ROWS = T::FM / PHASES ? T::FM / PHASES : 1; // 8-bit: fragment rows of a phase
+        if (T::PHASED && wm == 1)
+            turn();
         for (int stage = 0; stage < s.stages; ++stage) {
-            request_b();
-            request_a();
             const uint32_t a_at = at + slot_a * T::A_BYTES + wm * (T::FM * 16 * STAGE) + lane_at;
             const uint32_t b_at = at + T::B_AT + slot_b * T::B_BYTES + wn * (T::FN * 16 * STAGE) + lane_at;
-            u32x4 b[T::FN][2];
+            const unsigned char *scales = lds + T::SCALES_AT + slot_a * T::SCALE_BYTES;
+            const int next = stage + 1 < s.stages ? stage + 1 : 0; // of this tile or the block's next
+            const bool next_is_tail = tail && next + 1 == s.stages;
+            const int next_a = slot_a + 1 == T::AR ? 0 : slot_a + 1, next_b = slot_b ^ 1;
+            if constexpr (T::PHASED) {
+                if constexpr (T::E4M3) {
+                    i32x8 b[T::FN];
+                    float column;
 #pragma unroll
-            for (int j = 0; j < T::FN; ++j) {
-                b[j][0] = chunk_at(b_at + j * 2048);
-                b[j][1] = chunk_at((b_at + j * 2048) ^ 64);
-            }
-            if constexpr (T::E4M3) {
-                const unsigned char *scales = lds + T::SCALES_AT + slot_a * T::SCALE_BYTES;
-                const float column = *reinterpret_cast<const float *>(scales + T::BM * 4 + ((wn * 64) >> 7) * 4);
+                    for (int phase = 0; phase < PHASES; ++phase) {
+                        if (phase == 0) {
+                            column = *reinterpret_cast<const float *>(scales + T::BM * 4 + ((wn * 64) >> 7) * 4);
 #pragma unroll
-                for (int i = 0; i < T::FM; ++i) {
-                    const u32x4 low = chunk_at(a_at + i * 2048), high = chunk_at((a_at + i * 2048) ^ 64);
-                    const float scale = column * *reinterpret_cast<const float *>(scales + (wm * T::FM * 16 + i * 16 + (lane & 15)) * 4);
-                    const i32x8 a = __builtin_bit_cast(i32x8, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
+                            for (int j = 0; j < T::FN; ++j)
+                                b[j] = block_at(b_at + j * 2048);
+                        }
+                        i32x8 a[ROWS];
+                        float scale[ROWS];
 #pragma unroll
-                    for (int j = 0; j < T::FN; ++j) {
-                        const i32x8 w = __builtin_bit_cast(i32x8, __builtin_shufflevector(b[j][0], b[j][1], 0, 1, 2, 3, 4, 5, 6, 7));
-                        const f32x4 part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, f32x4{0, 0, 0, 0}, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+                        for (int i = 0; i < ROWS; ++i) {
+                            const int row = phase * ROWS + i;
+                            a[i] = block_at(a_at + row * 2048);
+                            scale[i] = *reinterpret_cast<const float *>(scales + (wm * T::FM * 16 + row * 16 + (lane & 15)) * 4);
+                        }
+                        if (phase == 0)
+                            request_b();
+                        if (phase == 1)
+                            request_a();
+                        if (phase == PHASES - 1 && wm == 1)
+                            landed(next_is_tail, next_a, next_b);
+                        turn();
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            acc[i][j][e] = fmaf(part[e], scale, acc[i][j][e]);
+                        for (int i = 0; i < ROWS; ++i)
+                            scale[i] *= column;
+                        __builtin_amdgcn_s_setprio(1);
+                        // a product is scaled and added two products later: one product's time is less than the matrix pipe's latency
+                        f32x4 part[3];
+#pragma unroll
+                        for (int n = 0; n < ROWS * T::FN + 2; ++n) {
+                            if (n < ROWS * T::FN)
+                                part[n % 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[n % T::FN], a[n / T::FN], f32x4{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+                            __builtin_amdgcn_sched_barrier(0);
+                            if (n >= 2) {
+                                const int d = n - 2;
+                                f32x4 &sum = acc[phase * ROWS + d / T::FN][d % T::FN];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    sum[e] = fmaf(part[d % 3][e], scale[d / T::FN], sum[e]);
+                            }
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+#pragma unroll
+                        for (int n = 0; n < ROWS * T::FN; ++n)
+                            pin(acc[phase * ROWS + n / T::FN][n % T::FN]);
+                        __builtin_amdgcn_s_setprio(0);
+                        if (phase == PHASES - 1 && wm == 0)
+                            landed(next_is_tail, next_a, next_b);
+                        turn();
+                    }
+                } else {
+#pragma unroll
+                    for (int phase = 0; phase < 2; ++phase) {
+                        const int flip = phase * 64;
+                        bf16x8 a[T::FM], b[T::FN];
+#pragma unroll
+                        for (int j = 0; j < T::FN; ++j)
+                            b[j] = __builtin_bit_cast(bf16x8, chunk_at((b_at + j * 2048) ^ flip));
+#pragma unroll
+                        for (int i = 0; i < T::FM; ++i)
+                            a[i] = __builtin_bit_cast(bf16x8, chunk_at((a_at + i * 2048) ^ flip));
+                        if (phase == 0)
+                            request_b();
+                        else {
+                            request_a();
+                            if (wm == 1)
+                                landed(next_is_tail, next_a, next_b);
+                        }
+                        turn();
+                        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                        for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+                            for (int j = 0; j < T::FN; ++j)
+                                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+                            for (int j = 0; j < T::FN; ++j)
+                                pin(acc[i][j]);
+                        __builtin_amdgcn_s_setprio(0);
+                        if (phase == 1 && wm == 0)
+                            landed(next_is_tail, next_a, next_b);
+                        turn();
                     }
                 }
             } else {
+                request_b();
+                request_a();
+                u32x4 b[T::FN][2];
 #pragma unroll
-                for (int i = 0; i < T::FM; ++i) {
-                    const bf16x8 low = __builtin_bit_cast(bf16x8, chunk_at(a_at + i * 2048));
-                    const bf16x8 high = __builtin_bit_cast(bf16x8, chunk_at((a_at + i * 2048) ^ 64));
+                for (int j = 0; j < T::FN; ++j) {
+                    b[j][0] = chunk_at(b_at + j * 2048);
+                    b[j][1] = chunk_at((b_at + j * 2048) ^ 64);
+                }
+                if constexpr (T::E4M3) {
+                    const float column = *reinterpret_cast<const float *>(scales + T::BM * 4 + ((wn * 64) >> 7) * 4);
 #pragma unroll
-                    for (int j = 0; j < T::FN; ++j) {
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b[j][0]), low, acc[i][j], 0, 0, 0);
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b[j][1]), high, acc[i][j], 0, 0, 0);
+                    for (int i = 0; i < T::FM; ++i) {
+                        const float scale = column * *reinterpret_cast<const float *>(scales + (wm * T::FM * 16 + i * 16 + (lane & 15)) * 4);
+                        const i32x8 a = block_at(a_at + i * 2048);
+#pragma unroll
+                        for (int j = 0; j < T::FN; ++j) {
+                            const i32x8 w = __builtin_bit_cast(i32x8, __builtin_shufflevector(b[j][0], b[j][1], 0, 1, 2, 3, 4, 5, 6, 7));
+                            const f32x4 part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, f32x4{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                acc[i][j][e] = fmaf(part[e], scale, acc[i][j][e]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < T::FM; ++i) {
+                        const bf16x8 low = __builtin_bit_cast(bf16x8, chunk_at(a_at + i * 2048));
+                        const bf16x8 high = __builtin_bit_cast(bf16x8, chunk_at((a_at + i * 2048) ^ 64));
+#pragma unroll
+                        for (int j = 0; j < T::FN; ++j) {
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b[j][0]), low, acc[i][j], 0, 0, 0);
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b[j][1]), high, acc[i][j], 0, 0, 0);
+                        }
                     }
                 }
             }
-            const int read_b = slot_b;
-            slot_a = slot_a + 1 == T::AR ? 0 : slot_a + 1;
-            slot_b ^= 1;
-            const int next = stage + 1 < s.stages ? stage + 1 : 0; // of this tile or the block's next
-            publish(tail && next + 1 == s.stages, slot_a, slot_b);
-            if (stage + 1 == s.stages) {
-                // every wave has left B's slot that was read, and no copy into it has been requested yet
-                epilogue.template finish<T>(s, acc, lds + T::B_AT + read_b * T::B_BYTES + wave * T::STAGING_BYTES, tile / s.tiles_n * T::BM + wm * T::FM * 16,
-                                            tile % s.tiles_n * T::COLUMNS + wn * (T::COLUMNS / T::WN), lane);
-                wait_lgkmcnt0();
-                __builtin_amdgcn_s_barrier(); // the next stage's copies go into that slot
-                asm volatile("" ::: "memory");
-            }
+            slot_a = next_a, slot_b = next_b;
+            if constexpr (!T::PHASED)
+                publish(next_is_tail, slot_a, slot_b);
         }
+        if (T::PHASED && wm == 0)
+            turn();
+        // every wave has left B's slot that was read last, and no copy into it has been requested yet
+        int tm, tn;
+        place(s, tile, tm, tn);
+        epilogue.template finish<T>(s, acc, lds + T::B_AT + (slot_b ^ 1) * T::B_BYTES + wave * T::STAGING_BYTES, tm * T::BM + wm * T::FM * 16, tn * T::COLUMNS + wn * (T::COLUMNS / T::WN), lane);
+        wait_lgkmcnt0();
+        turn(); // the next stage's copies go into that slot
     }
     wait_vmcnt<0>(); // no copy may land after the block's LDS has gone to another
 }
@@ -267,15 +393,19 @@ template <class T, class Epilogue> void launch_tiles(hipStream_t stream, Shape s
     static std::atomic<uint64_t> configured; // devices whose LDS opt-in for this kernel has been made
     int device = 0;
     check_hip(hipGetDevice(&device), "product: ");
-    if (!(configured.load(std::memory_order_acquire) >> (device & 63) & 1)) {
+    if (device > 63 || !(configured.load(std::memory_order_acquire) >> device & 1)) {
         check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(tile_kernel<T, Epilogue>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS_BYTES), "product LDS size: ");
-        configured.fetch_or(uint64_t(1) << (device & 63), std::memory_order_release);
+        if (device < 64)
+            configured.fetch_or(uint64_t(1) << device, std::memory_order_release);
     }
     hipLaunchKernelGGL((tile_kernel<T, Epilogue>), dim3(s.tiles < most ? s.tiles : most), dim3(T::THREADS), T::LDS_BYTES, stream, s, epilogue);
     check_hip(hipGetLastError(), "product launch: ");
 }
 template <bool E4M3, bool GATED, class Epilogue> void launch_product(hipStream_t stream, const Shape &s, const Epilogue &epilogue) {
-    launch_tiles<Tile<E4M3, GATED, 128, 128, 2, 2, 2>>(stream, s, epilogue);
+    if (int64_t(s.M) * s.N * (GATED ? 2 : 1) >= int64_t(256) * 256 * 200)
+        launch_tiles<Tile<E4M3, GATED, 256, 256, 2, 4, E4M3 ? 2 : 3, true>>(stream, s, epilogue);
+    else
+        launch_tiles<Tile<E4M3, GATED, 128, 128, 2, 2, 2>>(stream, s, epilogue);
 }
 
 } // namespace product

@@ -52,13 +52,21 @@ TG_DEVICE float largest8(const float (&v)[8]) {
 TG_DEVICE float scale_of(float largest) {
     return fmaxf(largest / LARGEST, LEAST_SCALE);
 }
-// RN_e4m3(v / scale): a true quotient, so that codes are those of the definition; |v / scale| <= 448 (1 + 2^-23), which rounds to 448
+// RN_e4m3(v / scale), of the correctly rounded quotient: v times the rounded reciprocal, put right by its own remainder (three
+// instructions where a division takes ten, and a lane has eight quotients).  |v / scale| <= 448 (1 + 2^-23), which rounds to 448.
 TG_DEVICE u32x2 encode8(const float (&v)[8], float scale) {
+    const float inverse = 1.0f / scale;
+    float quotient[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float first = v[e] * inverse;
+        quotient[e] = fmaf(fmaf(-first, scale, v[e]), inverse, first);
+    }
     u32x2 code;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-        int word = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * e] / scale, v[4 * e + 1] / scale, 0, false);
-        code[e] = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * e + 2] / scale, v[4 * e + 3] / scale, word, true));
+        int word = __builtin_amdgcn_cvt_pk_fp8_f32(quotient[4 * e], quotient[4 * e + 1], 0, false);
+        code[e] = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(quotient[4 * e + 2], quotient[4 * e + 3], word, true));
     }
     return code;
 }
@@ -75,54 +83,72 @@ template <int WAVES> TG_DEVICE float row_sum(float x, float *shared, int wave) {
     return (shared[0] + shared[1]) + (shared[2] + shared[3]);
 }
 
-template <int NC, int WAVES>
+// A block takes `each` rows that follow each other, so that what it writes of a group's scales lies side by side.  gamma is fetched once, and
+// a row's chunks while the row before is reduced.
+template <int NC, int WAVES, bool ADD>
 __global__ __launch_bounds__(256) void rmsnorm_fwd_kernel(const bf16_t *x, const bf16_t *residual, const uint16_t *__restrict__ gamma_hi,
                                                           const uint16_t *__restrict__ gamma_lo, bf16_t *sum, bf16_t *__restrict__ y,
-                                                          uint8_t *__restrict__ q, float *__restrict__ scales, int ld_scales, int rows, int D, float eps) {
+                                                          uint8_t *__restrict__ q, float *__restrict__ scales, int ld_scales, int rows, int each, int D, float eps) {
     constexpr int LANES = 64 * WAVES, SLOTS = 4 / WAVES;
     __shared__ float shared[4];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x % LANES, slot = threadIdx.x / LANES, chunks = D >> 3;
     const float inv_d = 1.0f / D;
-    for (int row0 = blockIdx.x * SLOTS; row0 < rows; row0 += gridDim.x * SLOTS) {
+    const int first = blockIdx.x * each, last = rows - first < each ? rows : first + each;
+    u32x4 raw[NC], add[NC];
+    const auto fetch = [&](int row) {
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+            const int c = lane + j * LANES;
+            raw[j] = add[j] = u32x4{0, 0, 0, 0};
+            if (row < last && c < chunks) {
+                raw[j] = *reinterpret_cast<const u32x4 *>(x + size_t(row) * D + c * 8);
+                if constexpr (ADD)
+                    add[j] = *reinterpret_cast<const u32x4 *>(residual + size_t(row) * D + c * 8);
+            }
+        }
+    };
+    fetch(first + slot);
+    float gamma[NC][8];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+        const int c = lane + j * LANES;
+        if (c < chunks)
+            join8(*reinterpret_cast<const u32x4 *>(gamma_hi + c * 8), *reinterpret_cast<const u32x4 *>(gamma_lo + c * 8), gamma[j]);
+    }
+    for (int row0 = first; row0 < last; row0 += SLOTS) {
         const int row = row0 + slot;
-        const bool live = row < rows;
+        const bool live = row < last;
         float v[NC][8];
         float squares = 0.f;
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             const int c = lane + j * LANES;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                v[j][e] = 0.f;
-            if (live && c < chunks) {
-                const size_t at = size_t(row) * D + c * 8;
-                unpack8(*reinterpret_cast<const u32x4 *>(x + at), v[j]);
-                if (residual) {
-                    float add[8];
-                    unpack8(*reinterpret_cast<const u32x4 *>(residual + at), add);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        v[j][e] += add[e];
-                    const u32x4 h = pack8(v[j]);
-                    *reinterpret_cast<u32x4 *>(sum + at) = h;
-                    unpack8(h, v[j]); // the norm is of what the next operators read
-                }
+            unpack8(raw[j], v[j]);
+            if constexpr (ADD) {
+                float other[8];
+                unpack8(add[j], other);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    squares = fmaf(v[j][e], v[j][e], squares);
+                    v[j][e] += other[e];
+                const u32x4 h = pack8(v[j]);
+                if (live && c < chunks)
+                    *reinterpret_cast<u32x4 *>(sum + size_t(row) * D + c * 8) = h;
+                unpack8(h, v[j]); // the norm is of what the next operators read
             }
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                squares = fmaf(v[j][e], v[j][e], squares);
         }
+        fetch(row + SLOTS); // in place of x or the residual, `sum` is written a row behind what is read
         const float inv = 1.0f / sqrtf(row_sum<WAVES>(squares, shared, wave) * inv_d + eps);
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             const int c = lane + j * LANES;
-            if (live && c < chunks) {
-                float gamma[8];
-                join8(*reinterpret_cast<const u32x4 *>(gamma_hi + c * 8), *reinterpret_cast<const u32x4 *>(gamma_lo + c * 8), gamma);
+            if (c < chunks) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    v[j][e] = v[j][e] * inv * gamma[e];
-                if (y)
+                    v[j][e] = v[j][e] * inv * gamma[j][e];
+                if (y && live)
                     *reinterpret_cast<u32x4 *>(y + size_t(row) * D + c * 8) = pack8(v[j]);
             }
             if (q) { // whole waves: lanes behind the last column hold zeros
@@ -137,15 +163,33 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_kernel(const bf16_t *x, const
     }
 }
 
-// dx, and a partial row of dgamma per slot into partial[block * SLOTS + slot][D]
+// dx, and a partial row of dgamma per block into partial[block][D].  Everything a row needs is requested while the row before is reduced.
 template <int NC, int WAVES>
 __global__ __launch_bounds__(256) void rmsnorm_bwd_kernel(const bf16_t *__restrict__ x, const bf16_t *__restrict__ dy, const uint16_t *__restrict__ gamma_hi,
                                                           const uint16_t *__restrict__ gamma_lo, const bf16_t *residual, bf16_t *dx,
                                                           float *__restrict__ partial, int rows, int D, float eps) {
     constexpr int LANES = 64 * WAVES, SLOTS = 4 / WAVES;
     __shared__ float shared[4];
+    extern __shared__ __attribute__((aligned(16))) float fold[]; // [SLOTS][D]
     const int wave = threadIdx.x >> 6, lane = threadIdx.x % LANES, slot = threadIdx.x / LANES, chunks = D >> 3;
     const float inv_d = 1.0f / D;
+    u32x4 raw_x[NC], raw_dy[NC], raw_add[NC];
+    const auto fetch = [&](int row) {
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+            const int c = lane + j * LANES;
+            raw_x[j] = raw_dy[j] = raw_add[j] = u32x4{0, 0, 0, 0};
+            if (row < rows && c < chunks) {
+                const size_t at = size_t(row) * D + c * 8;
+                raw_x[j] = *reinterpret_cast<const u32x4 *>(x + at);
+                raw_dy[j] = *reinterpret_cast<const u32x4 *>(dy + at);
+                if (residual) // may be dx: a row is read by the lanes that write it, before they do
+                    raw_add[j] = *reinterpret_cast<const u32x4 *>(residual + at);
+            }
+        }
+    };
+    const int step = gridDim.x * SLOTS;
+    fetch(blockIdx.x * SLOTS + slot);
     float gamma[NC][8], dgamma[NC][8];
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
@@ -156,101 +200,123 @@ __global__ __launch_bounds__(256) void rmsnorm_bwd_kernel(const bf16_t *__restri
         if (c < chunks)
             join8(*reinterpret_cast<const u32x4 *>(gamma_hi + c * 8), *reinterpret_cast<const u32x4 *>(gamma_lo + c * 8), gamma[j]);
     }
-    for (int row0 = blockIdx.x * SLOTS; row0 < rows; row0 += gridDim.x * SLOTS) {
+    for (int row0 = blockIdx.x * SLOTS; row0 < rows; row0 += step) {
         const int row = row0 + slot;
         const bool live = row < rows;
         float h[NC][8], t[NC][8];
+        u32x4 add[NC];
         float squares = 0.f, dot = 0.f;
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
-            const int c = lane + j * LANES;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                h[j][e] = t[j][e] = 0.f;
-            if (live && c < chunks) {
-                unpack8(*reinterpret_cast<const u32x4 *>(x + size_t(row) * D + c * 8), h[j]);
-                unpack8(*reinterpret_cast<const u32x4 *>(dy + size_t(row) * D + c * 8), t[j]);
-            }
+            unpack8(raw_x[j], h[j]);
+            unpack8(raw_dy[j], t[j]);
+            add[j] = raw_add[j];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 squares = fmaf(h[j][e], h[j][e], squares);
                 dot = fmaf(h[j][e], gamma[j][e] * t[j][e], dot);
             }
         }
+        fetch(row + step);
         const float inv = 1.0f / sqrtf(row_sum<WAVES>(squares, shared, wave) * inv_d + eps);
         const float pull = row_sum<WAVES>(dot, shared, wave) * inv_d * inv * inv; // of h, relative to gamma dy
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             const int c = lane + j * LANES;
             if (live && c < chunks) {
-                const size_t at = size_t(row) * D + c * 8;
-                float d[8];
+                float d[8], other[8];
+                unpack8(add[j], other); // zeros without a residual
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    d[e] = inv * (gamma[j][e] * t[j][e] - h[j][e] * pull);
+                    // the gradient through the norm and the residual's are added in 32 bits and rounded once
+                    d[e] = fmaf(inv, gamma[j][e] * t[j][e] - h[j][e] * pull, other[e]);
                     dgamma[j][e] = fmaf(t[j][e], h[j][e] * inv, dgamma[j][e]);
                 }
-                if (residual) { // added in 32 bits and rounded once
-                    float add[8];
-                    unpack8(*reinterpret_cast<const u32x4 *>(residual + at), add);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        d[e] += add[e];
-                }
-                *reinterpret_cast<u32x4 *>(dx + at) = pack8(d);
+                *reinterpret_cast<u32x4 *>(dx + size_t(row) * D + c * 8) = pack8(d);
             }
         }
     }
+    // the slots' sums, one on top of the other
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
         const int c = lane + j * LANES;
         if (c < chunks) {
-            float *to = partial + size_t(blockIdx.x * SLOTS + slot) * D + c * 8;
+            float *to = (SLOTS == 1 ? partial + size_t(blockIdx.x) * D : fold + slot * D) + c * 8;
             *reinterpret_cast<f32x4 *>(to) = f32x4{dgamma[j][0], dgamma[j][1], dgamma[j][2], dgamma[j][3]};
             *reinterpret_cast<f32x4 *>(to + 4) = f32x4{dgamma[j][4], dgamma[j][5], dgamma[j][6], dgamma[j][7]};
         }
     }
+    if constexpr (SLOTS > 1) {
+        __syncthreads();
+        for (int c = threadIdx.x * 4; c < D; c += 1024) {
+            f32x4 total = *reinterpret_cast<const f32x4 *>(fold + c);
+#pragma unroll
+            for (int k = 1; k < SLOTS; ++k)
+                total += *reinterpret_cast<const f32x4 *>(fold + k * D + c);
+            *reinterpret_cast<f32x4 *>(partial + size_t(blockIdx.x) * D + c) = total;
+        }
+    }
 }
 
-// the partial rows' sum in a fixed order: sixteen phases, each of every sixteenth row
+// the partial rows' sum in a fixed order: 32 phases, each of every 32nd row, eight of them in flight
 __global__ __launch_bounds__(256) void rmsnorm_bwd_reduce_kernel(const float *__restrict__ partial, int count, int D, float *__restrict__ dgamma, int accumulate) {
-    __shared__ float part[16][17];
-    const int col = threadIdx.x & 15, phase = threadIdx.x >> 4, i = blockIdx.x * 16 + col;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    if (i < D)
-        for (int b = phase; b < count; b += 64)
+    __shared__ float part[32][9];
+    const int col = threadIdx.x & 7, phase = threadIdx.x >> 3, i = blockIdx.x * 8 + col; // 8 divides D
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int b = phase; b < count; b += 256) {
+        float v[8];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (b + 16 * u < count)
-                    s[u] += partial[size_t(b + 16 * u) * D + i];
-    part[phase][col] = (s[0] + s[1]) + (s[2] + s[3]);
+        for (int u = 0; u < 8; ++u)
+            v[u] = b + 32 * u < count ? partial[size_t(b + 32 * u) * D + i] : 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            s[u] += v[u];
+    }
+    part[phase][col] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     __syncthreads();
-    if (phase == 0 && i < D) {
+    if (phase == 0) {
         float sum = 0.f;
 #pragma unroll
-        for (int p = 0; p < 16; ++p)
+        for (int p = 0; p < 32; ++p)
             sum += part[p][col];
         dgamma[i] = accumulate ? dgamma[i] + sum : sum;
     }
 }
 
-// a lane takes 8 columns, 16 lanes a group; a wave 512 columns of a row
+// A lane takes 8 columns, 16 lanes a group, a wave 512 columns of a row; a block 32 rows of them, four rows of a wave in flight, and writes their
+// scales side by side.
+constexpr int QUANTIZE_ROWS = 32;
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const bf16_t *__restrict__ x, int ldx, uint8_t *__restrict__ q, int ldq, float *__restrict__ scales,
                                                             int ld_scales, int rows, int columns, int parts) {
-    const int lane = threadIdx.x & 63;
-    const int64_t items = int64_t(rows) * parts;
-    for (int64_t item = blockIdx.x * 4 + (threadIdx.x >> 6); item < items; item += gridDim.x * 4) {
-        const int row = int(item / parts), c = (int(item % parts) * 64 + lane) * 8;
-        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (c < columns)
-            unpack8(*reinterpret_cast<const u32x4 *>(x + size_t(row) * ldx + c), v);
-        const float scale = scale_of(max_of_16(largest8(v)));
-        if (c < columns) {
-            *reinterpret_cast<u32x2 *>(q + size_t(row) * ldq + c) = encode8(v, scale);
+    __shared__ float shared[4][QUANTIZE_ROWS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int part = blockIdx.x % parts, first = blockIdx.x / parts * QUANTIZE_ROWS, c = (part * 64 + lane) * 8;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        u32x4 raw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = first + half * 16 + i * 4 + wave;
+            raw[i] = u32x4{0, 0, 0, 0};
+            if (row < rows && c < columns)
+                raw[i] = *reinterpret_cast<const u32x4 *>(x + size_t(row) * ldx + c);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int in = half * 16 + i * 4 + wave, row = first + in;
+            float v[8];
+            unpack8(raw[i], v);
+            const float scale = scale_of(max_of_16(largest8(v)));
+            if (row < rows && c < columns)
+                *reinterpret_cast<u32x2 *>(q + size_t(row) * ldq + c) = encode8(v, scale);
             if ((lane & 15) == 0)
-                scales[size_t(c >> 7) * ld_scales + row] = scale;
+                shared[lane >> 4][in] = scale;
         }
     }
+    __syncthreads();
+    const int group = threadIdx.x / QUANTIZE_ROWS, row = first + threadIdx.x % QUANTIZE_ROWS;
+    if (group < 4 && part * 512 + group * 128 < columns && row < rows)
+        scales[size_t(part * 4 + group) * ld_scales + row] = shared[group][threadIdx.x % QUANTIZE_ROWS];
 }
 
 // one block a tile of 128 x 128
@@ -295,9 +361,10 @@ void norm_shape(int rows, int D, float eps, const char *where) {
         throw std::invalid_argument(std::string(where) + ": rows at least 1, D a multiple of 8 and at most 8192, eps finite and not negative");
 }
 int slots_of(int D) { return D <= 2048 ? 4 : 1; } // rows a block works on at a time
-int forward_blocks(int rows, int D) {
-    const int need = (rows + slots_of(D) - 1) / slots_of(D);
-    return need < 2048 ? need : 2048;
+// rows a block takes in all: one round of its slots, more where that would be more than 1024 blocks
+int forward_rows(int rows, int D) {
+    const int slots = slots_of(D), rounds = (rows + 1024 * slots - 1) / (1024 * slots);
+    return rounds * slots;
 }
 int backward_blocks(int rows, int D) {
     const int need = (rows + 2 * slots_of(D) - 1) / (2 * slots_of(D));
@@ -337,15 +404,16 @@ extern "C" int tgk_rmsnorm_fwd(hipStream_t stream, int rows, int D, const uint16
             require(ld_scales >= rows, "rmsnorm_fwd: ld_scales must be at least the rows");
         }
         by_width(D, [&](auto nc, auto waves) {
-            hipLaunchKernelGGL((rmsnorm_fwd_kernel<nc(), waves()>), dim3(forward_blocks(rows, D)), dim3(256), 0, stream, x, residual, gamma_hi, gamma_lo, sum, y, q,
-                               scales, ld_scales, rows, D, eps);
+            const int each = forward_rows(rows, D), blocks = (rows - 1) / each + 1;
+            const auto kernel = residual ? rmsnorm_fwd_kernel<nc(), waves(), true> : rmsnorm_fwd_kernel<nc(), waves(), false>;
+            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, x, residual, gamma_hi, gamma_lo, sum, y, q, scales, ld_scales, rows, each, D, eps);
         });
         check_hip(hipGetLastError(), "rmsnorm_fwd launch: ");
     });
 }
 
 extern "C" size_t tgk_rmsnorm_bwd_workspace(int rows, int D) {
-    return rows > 0 && D > 0 && D <= MOST_D ? size_t(backward_blocks(rows, D)) * slots_of(D) * D * sizeof(float) : 0;
+    return rows > 0 && D > 0 && D <= MOST_D ? size_t(backward_blocks(rows, D)) * D * sizeof(float) : 0;
 }
 
 extern "C" int tgk_rmsnorm_bwd(hipStream_t stream, int rows, int D, const uint16_t *x, const uint16_t *dy, const uint16_t *gamma_hi, const uint16_t *gamma_lo,
@@ -365,9 +433,9 @@ extern "C" int tgk_rmsnorm_bwd(hipStream_t stream, int rows, int D, const uint16
         const int blocks = backward_blocks(rows, D);
         float *partial = static_cast<float *>(workspace);
         by_width(D, [&](auto nc, auto waves) {
-            hipLaunchKernelGGL((rmsnorm_bwd_kernel<nc(), waves()>), dim3(blocks), dim3(256), 0, stream, x, dy, gamma_hi, gamma_lo, residual, dx, partial, rows, D, eps);
+            hipLaunchKernelGGL((rmsnorm_bwd_kernel<nc(), waves()>), dim3(blocks), dim3(256), waves() == 1 ? 4 * D * sizeof(float) : 0, stream, x, dy, gamma_hi, gamma_lo, residual, dx, partial, rows, D, eps);
         });
-        hipLaunchKernelGGL(rmsnorm_bwd_reduce_kernel, dim3((D + 15) / 16), dim3(256), 0, stream, partial, blocks * slots_of(D), D, dgamma, accumulate);
+        hipLaunchKernelGGL(rmsnorm_bwd_reduce_kernel, dim3(D / 8), dim3(256), 0, stream, partial, blocks, D, dgamma, accumulate);
         check_hip(hipGetLastError(), "rmsnorm_bwd launch: ");
     });
 }
@@ -380,9 +448,10 @@ extern "C" int tgk_quantize_rows(hipStream_t stream, int rows, int columns, cons
         pointer(scales, 4, "quantize_rows: scales");
         require(ldx >= columns && ldx % 8 == 0 && ldq >= columns && ldq % 8 == 0, "quantize_rows: leading dimensions must be multiples of 8, at least the columns");
         require(ld_scales >= rows, "quantize_rows: ld_scales must be at least the rows");
-        const int parts = (columns + 511) / 512;
-        const int64_t need = (int64_t(rows) * parts + 3) / 4;
-        hipLaunchKernelGGL(quantize_rows_kernel, dim3(need < 4096 ? int(need) : 4096), dim3(256), 0, stream, x, ldx, q, ldq, scales, ld_scales, rows, columns, parts);
+        const int parts = (columns - 1) / 512 + 1;
+        const int64_t blocks = int64_t((rows - 1) / QUANTIZE_ROWS + 1) * parts;
+        require(blocks < (int64_t(1) << 30), "quantize_rows: too many rows and columns");
+        hipLaunchKernelGGL(quantize_rows_kernel, dim3(int(blocks)), dim3(256), 0, stream, x, ldx, q, ldq, scales, ld_scales, rows, columns, parts);
         check_hip(hipGetLastError(), "quantize_rows launch: ");
     });
 }
