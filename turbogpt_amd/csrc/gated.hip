@@ -59,6 +59,17 @@ template <int ACT, bool KEEP> struct GatedForward {
             }
         }
     }
+    template <int> TG_DEVICE void finish4(const Shape &s, const f32x4 (&sum)[2], int m, int n) const {
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            v[e] = act_f<ACT>(sum[0][e]) * sum[1][e];
+        *reinterpret_cast<u32x2 *>(h + size_t(m) * ld_h + n) = pack4(v);
+        if constexpr (KEEP) {
+            *reinterpret_cast<u32x2 *>(gu + size_t(m) * ld_gu + n) = pack4(sum[0]);
+            *reinterpret_cast<u32x2 *>(gu + size_t(m) * ld_gu + s.N + n) = pack4(sum[1]);
+        }
+    }
 };
 
 template <int ACT> struct GatedBackward {
@@ -90,6 +101,17 @@ template <int ACT> struct GatedBackward {
             }
         }
     }
+    template <int> TG_DEVICE void finish4(const Shape &s, const f32x4 (&dh)[1], int m, int n) const {
+        f32x4 g = unpack4(*reinterpret_cast<const u32x2 *>(gu + size_t(m) * ld_gu + n)), u = unpack4(*reinterpret_cast<const u32x2 *>(gu + size_t(m) * ld_gu + s.N + n));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const Gate gate = gate_f<ACT>(g[e]);
+            g[e] = dh[0][e] * u[e] * gate.slope;
+            u[e] = dh[0][e] * gate.act;
+        }
+        *reinterpret_cast<u32x2 *>(dgu + size_t(m) * ld_dgu + n) = pack4(g);
+        *reinterpret_cast<u32x2 *>(dgu + size_t(m) * ld_dgu + s.N + n) = pack4(u);
+    }
 };
 
 struct Plain {
@@ -109,6 +131,9 @@ struct Plain {
                     *reinterpret_cast<u32x4 *>(out + size_t(m) * ld_out + n) = pack8(v);
             }
         }
+    }
+    template <int> TG_DEVICE void finish4(const Shape &, const f32x4 (&sum)[1], int m, int n) const {
+        *reinterpret_cast<u32x2 *>(out + size_t(m) * ld_out + n) = pack4(sum[0]);
     }
 };
 

@@ -35,6 +35,12 @@ template <bool ADD> struct Residual {
             }
         }
     }
+    template <int> TG_DEVICE void finish4(const Shape &, const f32x4 (&sum)[1], int m, int n) const {
+        f32x4 v = sum[0];
+        if constexpr (ADD)
+            v += unpack4(*reinterpret_cast<const u32x2 *>(residual + size_t(m) * ld_residual + n));
+        *reinterpret_cast<u32x2 *>(out + size_t(m) * ld_out + n) = pack4(v);
+    }
 };
 
 void operand(const void *p, int ld, int columns, int unit, const char *what) {

@@ -10,30 +10,15 @@
 // operands; chunks behind the end of k are read from the stage's first chunk and overwritten with zeros in both operands
 // before the stage is published, as what lies behind a row's end may be anything, NaN included.
 #pragma once
-#include "common.h"
-#include <atomic>
-#include <type_traits>
+#include "product_few.h"
 
 namespace product {
 
-constexpr int STAGE = 128; // bytes of k
-
-struct Shape {
-    const unsigned char *a, *b;
-    int64_t lda, ldb;    // bytes from row to row
-    int M, N;            // rows of a; rows of b, or (gated) half of them: columns of the result
-    int k_bytes, stages; // stages = ceil(k_bytes / STAGE)
-    int tiles_m, tiles_n, tiles;
-    const float *a_scales, *b_scales; // of 8-bit operands: [stage][ld_a_scales] by row, [row / 128][ld_b_scales] by stage
-    int ld_a_scales, ld_b_scales;
-};
-
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
-// WM x WN waves of (BM / WM) x 64 outputs.  AR: slots of A's ring (2 or 3; B's has 2), a stage of A is requested AR - 1
-// stages ahead.  GATED: B's rows are of two matrices on top of each other, N rows each; every wave's 64 are 32 of the upper
+// WM x WN waves of (BM / WM) x 64 outputs.  AR and BR: slots of A's and B's rings; a stage is requested one less than that ahead.
+// PHASED: the two halves of the waves take turns (below), B's ring has two slots; otherwise both rings have as many.  GATED: B's rows are of two matrices on top of each other, N rows each; every wave's 64 are 32 of the upper
 // and the same 32 of the lower, and a tile has BN / 2 columns of the result.
 template <bool E4M3_, bool GATED_, int BM_, int BN_, int WM_, int WN_, int AR_, bool PHASED_ = false> struct Tile {
+    static constexpr int BR = PHASED_ ? 2 : AR_;
     static constexpr bool E4M3 = E4M3_, GATED = GATED_, PHASED = PHASED_;
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, AR = AR_, WAVES = WM * WN, THREADS = WAVES * 64;
     static constexpr int FM = BM / WM / 16, FN = 4, COLUMNS = GATED ? BN / 2 : BN;
@@ -41,7 +26,7 @@ template <bool E4M3_, bool GATED_, int BM_, int BN_, int WM_, int WN_, int AR_, 
     static constexpr int A_BYTES = BM * STAGE, B_BYTES = BN * STAGE;
     static constexpr int SCALE_BYTES = E4M3 ? BM * 4 + 256 : 0; // a slot: the rows' scales, then 64 floats of the columns'
     static constexpr int STAGING_BYTES = 4096;                  // a wave's 16 x 64 results
-    static constexpr int B_AT = AR * A_BYTES, SCALES_AT = B_AT + 2 * B_BYTES, LDS_BYTES = SCALES_AT + AR * SCALE_BYTES;
+    static constexpr int B_AT = AR * A_BYTES, SCALES_AT = B_AT + BR * B_BYTES, LDS_BYTES = SCALES_AT + AR * SCALE_BYTES;
     static_assert(BN / WN == 64 && BN <= 256 && BM / 64 <= WAVES / (E4M3 ? 2 : 1) && B_BYTES >= WAVES * STAGING_BYTES, "tile");
 };
 
@@ -60,15 +45,6 @@ TG_DEVICE void staged8(const unsigned char *staging, int r, int q, float (&v)[8]
     for (int e = 0; e < 4; ++e)
         v[e] = lo[e], v[4 + e] = hi[e];
 }
-TG_DEVICE u32x4 pack8(const float (&v)[8]) {
-    return u32x4{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
-}
-TG_DEVICE void unpack8(const u32x4 &p, float (&v)[8]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        v[2 * e] = bf16_lo(p[e]), v[2 * e + 1] = bf16_hi(p[e]);
-}
-
 // Tiles are walked in bands of four rows of tiles, column by column: 32 neighbours, what an XCD works on at a time, are 4 x 8 tiles
 // and share 12 panels of the operands in its L2, where 32 in one row would share 33.
 constexpr int BAND = 4;
@@ -148,7 +124,7 @@ template <class T, bool IS_A> struct Producer {
             *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(slot_at + (j * T::WAVES + wave) * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
     }
     TG_DEVICE void advance(const Shape &s, int step, int wave, int lane) {
-        slot = slot + 1 == (IS_A ? T::AR : 2) ? 0 : slot + 1;
+        slot = slot + 1 == (IS_A ? T::AR : T::BR) ? 0 : slot + 1;
         if (stage + 1 < s.stages)
             ++stage;
         else if (tile + step < s.tiles) // otherwise the last stage again: the number of copies in flight stays the same
@@ -190,11 +166,15 @@ void tile_kernel(Shape s, Epilogue epilogue) {
     };
     request_b();
     request_a();
-    if constexpr (T::AR == 3)
+#pragma unroll
+    for (int ahead = 2; ahead < T::AR; ++ahead) {
+        if (!T::PHASED)
+            request_b();
         request_a();
+    }
     const int tail = (s.k_bytes % STAGE + 15) >> 4; // chunks of the last stage, 0: all
     const auto landed = [&](bool is_tail, int slot_a, int slot_b) {
-        wait_vmcnt<T::AR == 3 ? T::A_COPIES + T::SCALE_COPIES : 0>();
+        wait_vmcnt<(T::AR - 2) * (T::A_COPIES + T::SCALE_COPIES + (T::PHASED ? 0 : T::B_COPIES))>();
         if (is_tail) {
             Producer<T, true>::clear_tail(at + slot_a * T::A_BYTES, tail, wave, lane);
             Producer<T, false>::clear_tail(at + T::B_AT + slot_b * T::B_BYTES, tail, wave, lane);
@@ -237,7 +217,7 @@ void tile_kernel(Shape s, Epilogue epilogue) {
             const unsigned char *scales = lds + T::SCALES_AT + slot_a * T::SCALE_BYTES;
             const int next = stage + 1 < s.stages ? stage + 1 : 0; // of this tile or the block's next
             const bool next_is_tail = tail && next + 1 == s.stages;
-            const int next_a = slot_a + 1 == T::AR ? 0 : slot_a + 1, next_b = slot_b ^ 1;
+            const int next_a = slot_a + 1 == T::AR ? 0 : slot_a + 1, next_b = slot_b + 1 == T::BR ? 0 : slot_b + 1;
             if constexpr (T::PHASED) {
                 if constexpr (T::E4M3) {
                     i32x8 b[T::FN];
@@ -375,7 +355,7 @@ void tile_kernel(Shape s, Epilogue epilogue) {
         // every wave has left B's slot that was read last, and no copy into it has been requested yet
         int tm, tn;
         place(s, tile, tm, tn);
-        epilogue.template finish<T>(s, acc, lds + T::B_AT + (slot_b ^ 1) * T::B_BYTES + wave * T::STAGING_BYTES, tm * T::BM + wm * T::FM * 16, tn * T::COLUMNS + wn * (T::COLUMNS / T::WN), lane);
+        epilogue.template finish<T>(s, acc, lds + T::B_AT + (slot_b ? slot_b - 1 : T::BR - 1) * T::B_BYTES + wave * T::STAGING_BYTES, tm * T::BM + wm * T::FM * 16, tn * T::COLUMNS + wn * (T::COLUMNS / T::WN), lane);
         wait_lgkmcnt0();
         turn(); // the next stage's copies go into that slot
     }
@@ -390,22 +370,49 @@ template <class T, class Epilogue> void launch_tiles(hipStream_t stream, Shape s
     require(int64_t(s.tiles_m) * s.tiles_n < (int64_t(1) << 30), "product: too many tiles");
     s.tiles = s.tiles_m * s.tiles_n, s.stages = (s.k_bytes + STAGE - 1) / STAGE;
     const int most = T::LDS_BYTES > 81920 ? 256 : 512;
-    static std::atomic<uint64_t> configured; // devices whose LDS opt-in for this kernel has been made
-    int device = 0;
-    check_hip(hipGetDevice(&device), "product: ");
-    if (device > 63 || !(configured.load(std::memory_order_acquire) >> device & 1)) {
-        check_hip(hipFuncSetAttribute(reinterpret_cast<const void *>(tile_kernel<T, Epilogue>), hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS_BYTES), "product LDS size: ");
-        if (device < 64)
-            configured.fetch_or(uint64_t(1) << device, std::memory_order_release);
-    }
+    static std::atomic<uint64_t> configured;
+    allow_lds(tile_kernel<T, Epilogue>, configured, T::LDS_BYTES);
     hipLaunchKernelGGL((tile_kernel<T, Epilogue>), dim3(s.tiles < most ? s.tiles : most), dim3(T::THREADS), T::LDS_BYTES, stream, s, epilogue);
     check_hip(hipGetLastError(), "product launch: ");
 }
-template <bool E4M3, bool GATED, class Epilogue> void launch_product(hipStream_t stream, const Shape &s, const Epilogue &epilogue) {
-    if (int64_t(s.M) * s.N * (GATED ? 2 : 1) >= int64_t(256) * 256 * 200)
+// Which kernel.  While 256 blocks, one a unit, cover the result, the smallest of the few kernel's shapes that does it (its blocks share out k, so one
+// is never worse than more: 1000 columns, K = 1904 in 8 bits, 1024 rows 11.3 us, tiles of 64 x 128 14.3; at 2048 rows, 512 blocks, 18 and 15.2).
+// Otherwise the least of the tiles' estimated times, us: per stage a tile's time alone on its unit, or of two (of 256 x 256 it grows with the
+// share of units that have one, as all of them ask the same memory), and an epilogue; fitted to the operators at 64 to 16384 rows.  Gated, 2 x 2816
+// columns, D = 1024, on 64 x 128, 128 x 128, 256 x 256: 512 rows 15.8, 17.7, 26; 1024 28.9, 20.7, 27.5; 2048 40, 40, 30.
+struct TileTimes {
+    double alone, two, epilogue;
+};
+inline double tiles_us(int64_t tiles, int stages, const TileTimes &t) {
+    const int64_t rounds = tiles / 512, rest = tiles % 512;
+    return rounds * (stages * t.two + t.epilogue) + (rest > 256 ? stages * t.two + t.epilogue : rest ? stages * t.alone + t.epilogue : 0.0);
+}
+inline double large_tiles_us(int64_t tiles, int stages, const TileTimes &t) { // `two`: alone, with every unit at work
+    const int64_t rounds = tiles / 256, rest = tiles % 256;
+    return rounds * (stages * t.two + t.epilogue) + (rest ? stages * (t.alone + (t.two - t.alone) * (rounds ? 1.0 : rest / 256.0)) + t.epilogue : 0.0);
+}
+template <bool E4M3, bool GATED, class Epilogue> void launch_product(hipStream_t stream, Shape s, const Epilogue &epilogue) {
+    s.stages = (s.k_bytes + STAGE - 1) / STAGE;
+    const auto count = [&](int rows, int columns) { return int64_t((s.M + rows - 1) / rows) * ((s.N + columns - 1) / columns); };
+    if (count(16, 16) <= 256)
+        return launch_few<Few<E4M3, GATED, 1, 1, 2>>(stream, s, epilogue);
+    if (count(32, 32) <= 256)
+        return launch_few<Few<E4M3, GATED, 2, 2, 1>>(stream, s, epilogue);
+    if (count(64, 32) <= 256)
+        return launch_few<Few<E4M3, GATED, 4, 2, 1>>(stream, s, epilogue);
+    if constexpr (!GATED)
+        if (count(64, 64) <= 256)
+            return launch_few<Few<E4M3, GATED, 4, 4, 1>>(stream, s, epilogue);
+    constexpr int OF = GATED ? 2 : 1; // a tile's columns of B for one of the result
+    const double low = tiles_us(count(64, 128 / OF), s.stages, E4M3 ? TileTimes{0.54, 0.90, 1.5} : TileTimes{0.42, 0.72, 1.5});
+    const double square = tiles_us(count(128, 128 / OF), s.stages, E4M3 ? TileTimes{0.77, 1.25, 2.5} : TileTimes{0.57, 1.10, 2.5});
+    const double large = large_tiles_us(count(256, 256 / OF), s.stages, E4M3 ? TileTimes{1.65, 1.90, 6.0} : TileTimes{0.95, 1.58, 6.0});
+    if (large <= low && large <= square)
         launch_tiles<Tile<E4M3, GATED, 256, 256, 2, 4, E4M3 ? 2 : 3, true>>(stream, s, epilogue);
-    else
+    else if (square <= low)
         launch_tiles<Tile<E4M3, GATED, 128, 128, 2, 2, 2>>(stream, s, epilogue);
+    else
+        launch_tiles<Tile<E4M3, GATED, 64, 128, 2, 2, 3>>(stream, s, epilogue);
 }
 
 } // namespace product
