@@ -37,7 +37,7 @@ template <int ACT, bool KEEP> struct GatedForward {
     int ld_h, ld_gu;
     // The activation and the product are taken of the 32-bit sums and rounded once; what is kept for the backward pass is
     // rounded by itself.
-    template <class T> TG_DEVICE void finish(const Shape &s, const f32x4 (&acc)[T::FM][T::FN], unsigned char *staging, int m_base, int n_base, int lane) const {
+    template <class T, bool INSIDE> TG_DEVICE void finish(const Shape &s, const f32x4 (&acc)[T::FM][T::FN], unsigned char *staging, int m_base, int n_base, int lane) const {
         const int r = lane >> 2, q = lane & 3, f = n_base + q * 8;
 #pragma unroll
         for (int i = 0; i < T::FM; ++i) {
@@ -47,7 +47,7 @@ template <int ACT, bool KEEP> struct GatedForward {
             staged8(staging, r, q, g);
             staged8(staging, r, 4 + q, u);
             const int m = m_base + i * 16 + r;
-            if (m < s.M && f < s.N) {
+            if (INSIDE || (m < s.M && f < s.N)) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     v[e] = act_f<ACT>(g[e]) * u[e];
@@ -76,19 +76,38 @@ template <int ACT> struct GatedBackward {
     const bf16_t *gu; // may be dgu: every lane reads its values before it writes them
     bf16_t *dgu;
     int ld_gu, ld_dgu;
-    template <class T> TG_DEVICE void finish(const Shape &s, const f32x4 (&acc)[T::FM][T::FN], unsigned char *staging, int m_base, int n_base, int lane) const {
+    // The saved pre-activations of AHEAD fragment rows are on their way while one is finished.
+    template <class T, bool INSIDE> TG_DEVICE void finish(const Shape &s, const f32x4 (&acc)[T::FM][T::FN], unsigned char *staging, int m_base, int n_base, int lane) const {
+        constexpr int AHEAD = T::FM < 3 ? T::FM : 3;
+        const int r = lane >> 3, q = lane & 7, f = n_base + q * 8;
+        u32x4 raw[AHEAD][2][2];
+        const auto fetch = [&](int i) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int m = m_base + i * 16 + half * 8 + r;
+                if (INSIDE || (m < s.M && f < s.N)) {
+                    const bf16_t *from = gu + size_t(m) * ld_gu + f;
+                    // read once and larger than the L2s, whose lines the operands need: 16384 x 4096, D = 1024 196 us through them, 184 past them
+                    raw[i % AHEAD][half][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(from));
+                    raw[i % AHEAD][half][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(from + s.N));
+                }
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            fetch(i);
 #pragma unroll
         for (int i = 0; i < T::FM; ++i) {
             __builtin_amdgcn_sched_barrier(0); // one fragment row at a time: hoisted loads would not leave the sums their registers
             stage_results<T>(acc[i], staging, lane);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const int r = (lane >> 3) + half * 8, q = lane & 7, m = m_base + i * 16 + r, f = n_base + q * 8;
+                const int m = m_base + i * 16 + half * 8 + r;
                 float dh[8], g[8], u[8];
-                staged8(staging, r, q, dh);
-                if (m < s.M && f < s.N) {
-                    unpack8(*reinterpret_cast<const u32x4 *>(gu + size_t(m) * ld_gu + f), g);
-                    unpack8(*reinterpret_cast<const u32x4 *>(gu + size_t(m) * ld_gu + s.N + f), u);
+                staged8(staging, half * 8 + r, q, dh);
+                if (INSIDE || (m < s.M && f < s.N)) {
+                    unpack8(raw[i % AHEAD][half][0], g);
+                    unpack8(raw[i % AHEAD][half][1], u);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const Gate gate = gate_f<ACT>(g[e]);
@@ -99,6 +118,8 @@ template <int ACT> struct GatedBackward {
                     *reinterpret_cast<u32x4 *>(dgu + size_t(m) * ld_dgu + s.N + f) = pack8(u);
                 }
             }
+            if (i + AHEAD < T::FM)
+                fetch(i + AHEAD);
         }
     }
     template <int> TG_DEVICE void finish4(const Shape &s, const f32x4 (&dh)[1], int m, int n) const {
@@ -117,7 +138,7 @@ template <int ACT> struct GatedBackward {
 struct Plain {
     bf16_t *out;
     int ld_out;
-    template <class T> TG_DEVICE void finish(const Shape &s, const f32x4 (&acc)[T::FM][T::FN], unsigned char *staging, int m_base, int n_base, int lane) const {
+    template <class T, bool INSIDE> TG_DEVICE void finish(const Shape &s, const f32x4 (&acc)[T::FM][T::FN], unsigned char *staging, int m_base, int n_base, int lane) const {
 #pragma unroll
         for (int i = 0; i < T::FM; ++i) {
             __builtin_amdgcn_sched_barrier(0); // one fragment row at a time: hoisted loads would not leave the sums their registers
@@ -127,7 +148,7 @@ struct Plain {
                 const int r = (lane >> 3) + half * 8, q = lane & 7, m = m_base + i * 16 + r, n = n_base + q * 8;
                 float v[8];
                 staged8(staging, r, q, v);
-                if (m < s.M && n < s.N)
+                if (INSIDE || (m < s.M && n < s.N))
                     *reinterpret_cast<u32x4 *>(out + size_t(m) * ld_out + n) = pack8(v);
             }
         }

@@ -13,19 +13,35 @@ template <bool ADD> struct Residual {
     bf16_t *out;
     const bf16_t *residual;
     int ld_out, ld_residual;
-    template <class T> TG_DEVICE void finish(const Shape &s, const f32x4 (&acc)[T::FM][T::FN], unsigned char *staging, int m_base, int n_base, int lane) const {
+    // The residual (may be the output itself: every lane reads its values before it writes them) of AHEAD fragment rows is on its way while one is finished.
+    template <class T, bool INSIDE> TG_DEVICE void finish(const Shape &s, const f32x4 (&acc)[T::FM][T::FN], unsigned char *staging, int m_base, int n_base, int lane) const {
+        constexpr int AHEAD = T::FM < 3 ? T::FM : 3;
+        const int r = lane >> 3, q = lane & 7, n = n_base + q * 8;
+        u32x4 raw[AHEAD][2];
+        const auto fetch = [&](int i) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int m = m_base + i * 16 + half * 8 + r;
+                if (INSIDE || (m < s.M && n < s.N))
+                    raw[i % AHEAD][half] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(residual + size_t(m) * ld_residual + n)); // read once
+            }
+        };
+        if constexpr (ADD)
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                fetch(i);
 #pragma unroll
         for (int i = 0; i < T::FM; ++i) {
             __builtin_amdgcn_sched_barrier(0); // one fragment row at a time: hoisted loads would not leave the sums their registers
             stage_results<T>(acc[i], staging, lane);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const int r = (lane >> 3) + half * 8, q = lane & 7, m = m_base + i * 16 + r, n = n_base + q * 8;
+                const int m = m_base + i * 16 + half * 8 + r;
                 float v[8], add[8];
-                staged8(staging, r, q, v);
-                if (m < s.M && n < s.N) {
-                    if constexpr (ADD) { // in 32 bits, rounded once; may be the output itself: read before it is written
-                        unpack8(*reinterpret_cast<const u32x4 *>(residual + size_t(m) * ld_residual + n), add);
+                staged8(staging, half * 8 + r, q, v);
+                if (INSIDE || (m < s.M && n < s.N)) {
+                    if constexpr (ADD) { // in 32 bits, rounded once
+                        unpack8(raw[i % AHEAD][half], add);
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
                             v[e] += add[e];
@@ -33,6 +49,8 @@ template <bool ADD> struct Residual {
                     *reinterpret_cast<u32x4 *>(out + size_t(m) * ld_out + n) = pack8(v);
                 }
             }
+            if (ADD && i + AHEAD < T::FM)
+                fetch(i + AHEAD);
         }
     }
     template <int> TG_DEVICE void finish4(const Shape &, const f32x4 (&sum)[1], int m, int n) const {

@@ -355,7 +355,14 @@ void tile_kernel(Shape s, Epilogue epilogue) {
         // every wave has left B's slot that was read last, and no copy into it has been requested yet
         int tm, tn;
         place(s, tile, tm, tn);
-        epilogue.template finish<T>(s, acc, lds + T::B_AT + (slot_b ? slot_b - 1 : T::BR - 1) * T::B_BYTES + wave * T::STAGING_BYTES, tm * T::BM + wm * T::FM * 16, tn * T::COLUMNS + wn * (T::COLUMNS / T::WN), lane);
+        const int m_base = tm * T::BM + wm * T::FM * 16, n_base = tn * T::COLUMNS + wn * (T::COLUMNS / T::WN);
+        unsigned char *staging = lds + T::B_AT + (slot_b ? slot_b - 1 : T::BR - 1) * T::B_BYTES + wave * T::STAGING_BYTES;
+        // Without a branch where the wave's results are all inside: behind one, how many stores are in flight is not known, and every load would be
+        // awaited together with the stores before it.
+        if (m_base + T::FM * 16 <= s.M && n_base + T::COLUMNS / T::WN <= s.N)
+            epilogue.template finish<T, true>(s, acc, staging, m_base, n_base, lane);
+        else
+            epilogue.template finish<T, false>(s, acc, staging, m_base, n_base, lane);
         wait_lgkmcnt0();
         turn(); // the next stage's copies go into that slot
     }
