@@ -71,6 +71,16 @@ TG_DEVICE u32x2 encode8(const float (&v)[8], float scale) {
     return code;
 }
 
+// Results larger than the L2s together go past them (`past`), smaller ones stay for the next operator: 16384 x 2048 to 8 bits 50 us through them, 44
+// past; 16384 x 768 forward and backward, where the backward pass reads the sum again, 43.4 and 44.4.
+constexpr size_t LARGE_RESULT = size_t(32) << 20;
+template <bool PAST, class V> TG_DEVICE void store(void *to, const V &v) {
+    if constexpr (PAST)
+        __builtin_nontemporal_store(v, reinterpret_cast<V *>(to));
+    else
+        *reinterpret_cast<V *>(to) = v;
+}
+
 // WAVES waves a row, NC chunks of 8 columns a lane; a block of four waves takes 4 / WAVES rows at a time.
 template <int WAVES> TG_DEVICE float row_sum(float x, float *shared, int wave) {
     x = wave_sum(x);
@@ -85,7 +95,7 @@ template <int WAVES> TG_DEVICE float row_sum(float x, float *shared, int wave) {
 
 // A block takes `each` rows that follow each other, so that what it writes of a group's scales lies side by side.  gamma is fetched once, and
 // a row's chunks while the row before is reduced.
-template <int NC, int WAVES, bool ADD>
+template <int NC, int WAVES, bool ADD, bool PAST>
 __global__ __launch_bounds__(256) void rmsnorm_fwd_kernel(const bf16_t *x, const bf16_t *residual, const uint16_t *__restrict__ gamma_hi,
                                                           const uint16_t *__restrict__ gamma_lo, bf16_t *sum, bf16_t *__restrict__ y,
                                                           uint8_t *__restrict__ q, float *__restrict__ scales, int ld_scales, int rows, int each, int D, float eps) {
@@ -132,7 +142,7 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_kernel(const bf16_t *x, const
                     v[j][e] += other[e];
                 const u32x4 h = pack8(v[j]);
                 if (live && c < chunks)
-                    *reinterpret_cast<u32x4 *>(sum + size_t(row) * D + c * 8) = h;
+                    store<PAST>(sum + size_t(row) * D + c * 8, h);
                 unpack8(h, v[j]); // the norm is of what the next operators read
             }
 #pragma unroll
@@ -149,12 +159,12 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_kernel(const bf16_t *x, const
                 for (int e = 0; e < 8; ++e)
                     v[j][e] = v[j][e] * inv * gamma[j][e];
                 if (y && live)
-                    *reinterpret_cast<u32x4 *>(y + size_t(row) * D + c * 8) = pack8(v[j]);
+                    store<PAST>(y + size_t(row) * D + c * 8, pack8(v[j]));
             }
             if (q) { // whole waves: lanes behind the last column hold zeros
                 const float scale = scale_of(max_of_16(largest8(v[j])));
                 if (live && c < chunks) {
-                    *reinterpret_cast<u32x2 *>(q + size_t(row) * D + c * 8) = encode8(v[j], scale);
+                    store<PAST>(q + size_t(row) * D + c * 8, encode8(v[j], scale));
                     if ((c & 15) == 0)
                         scales[size_t(c >> 4) * ld_scales + row] = scale;
                 }
@@ -164,7 +174,7 @@ __global__ __launch_bounds__(256) void rmsnorm_fwd_kernel(const bf16_t *x, const
 }
 
 // dx, and a partial row of dgamma per block into partial[block][D].  Everything a row needs is requested while the row before is reduced.
-template <int NC, int WAVES>
+template <int NC, int WAVES, bool PAST>
 __global__ __launch_bounds__(256) void rmsnorm_bwd_kernel(const bf16_t *__restrict__ x, const bf16_t *__restrict__ dy, const uint16_t *__restrict__ gamma_hi,
                                                           const uint16_t *__restrict__ gamma_lo, const bf16_t *residual, bf16_t *dx,
                                                           float *__restrict__ partial, int rows, int D, float eps) {
@@ -232,7 +242,7 @@ __global__ __launch_bounds__(256) void rmsnorm_bwd_kernel(const bf16_t *__restri
                     d[e] = fmaf(inv, gamma[j][e] * t[j][e] - h[j][e] * pull, other[e]);
                     dgamma[j][e] = fmaf(t[j][e], h[j][e] * inv, dgamma[j][e]);
                 }
-                *reinterpret_cast<u32x4 *>(dx + size_t(row) * D + c * 8) = pack8(d);
+                store<PAST>(dx + size_t(row) * D + c * 8, pack8(d));
             }
         }
     }
@@ -361,14 +371,16 @@ void norm_shape(int rows, int D, float eps, const char *where) {
         throw std::invalid_argument(std::string(where) + ": rows at least 1, D a multiple of 8 and at most 8192, eps finite and not negative");
 }
 int slots_of(int D) { return D <= 2048 ? 4 : 1; } // rows a block works on at a time
-// rows a block takes in all: one round of its slots, more where that would be more than 1024 blocks
+// rows a block takes in all: one round of its slots, more where that would be more than 2048 blocks (16384 x 2048 to 8 bits 53 us with 1024, 50 with 2048)
 int forward_rows(int rows, int D) {
-    const int slots = slots_of(D), rounds = (rows + 1024 * slots - 1) / (1024 * slots);
+    const int slots = slots_of(D), rounds = (rows + 2048 * slots - 1) / (2048 * slots);
     return rounds * slots;
 }
+// two rounds of the slots at least, and at most two blocks a unit (16384 x 768, 1024, 2048: 23.6, 28.0, 58.2 us; with three 24.2, 29.2, 63.2; with four 25.9,
+// 32.6, 61.5)
 int backward_blocks(int rows, int D) {
     const int need = (rows + 2 * slots_of(D) - 1) / (2 * slots_of(D));
-    return need < 768 ? need : 768;
+    return need < 512 ? need : 512;
 }
 // f(chunks a lane, waves a row)
 template <class F> void by_width(int D, F &&f) {
@@ -405,7 +417,9 @@ extern "C" int tgk_rmsnorm_fwd(hipStream_t stream, int rows, int D, const uint16
         }
         by_width(D, [&](auto nc, auto waves) {
             const int each = forward_rows(rows, D), blocks = (rows - 1) / each + 1;
-            const auto kernel = residual ? rmsnorm_fwd_kernel<nc(), waves(), true> : rmsnorm_fwd_kernel<nc(), waves(), false>;
+            const bool past = size_t(rows) * D * 2 > LARGE_RESULT;
+            const auto kernel = past ? (residual ? rmsnorm_fwd_kernel<nc(), waves(), true, true> : rmsnorm_fwd_kernel<nc(), waves(), false, true>)
+                                     : (residual ? rmsnorm_fwd_kernel<nc(), waves(), true, false> : rmsnorm_fwd_kernel<nc(), waves(), false, false>);
             hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, x, residual, gamma_hi, gamma_lo, sum, y, q, scales, ld_scales, rows, each, D, eps);
         });
         check_hip(hipGetLastError(), "rmsnorm_fwd launch: ");
@@ -433,7 +447,8 @@ extern "C" int tgk_rmsnorm_bwd(hipStream_t stream, int rows, int D, const uint16
         const int blocks = backward_blocks(rows, D);
         float *partial = static_cast<float *>(workspace);
         by_width(D, [&](auto nc, auto waves) {
-            hipLaunchKernelGGL((rmsnorm_bwd_kernel<nc(), waves()>), dim3(blocks), dim3(256), waves() == 1 ? 4 * D * sizeof(float) : 0, stream, x, dy, gamma_hi, gamma_lo, residual, dx, partial, rows, D, eps);
+            const auto kernel = size_t(rows) * D * 2 > LARGE_RESULT ? rmsnorm_bwd_kernel<nc(), waves(), true> : rmsnorm_bwd_kernel<nc(), waves(), false>;
+            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), waves() == 1 ? 4 * D * sizeof(float) : 0, stream, x, dy, gamma_hi, gamma_lo, residual, dx, partial, rows, D, eps);
         });
         hipLaunchKernelGGL(rmsnorm_bwd_reduce_kernel, dim3(D / 8), dim3(256), 0, stream, partial, blocks, D, dgamma, accumulate);
         check_hip(hipGetLastError(), "rmsnorm_bwd launch: ");
