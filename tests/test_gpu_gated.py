@@ -15,7 +15,7 @@ SILU, GELU = 0, 1
 HALF = 2.0 ** -8
 ACT = 2.0 ** -19
 SHAPES = [(1, 8, 8), (1, 256, 128), (2, 1720, 640), (17, 72, 200), (64, 64, 64), (65, 136, 72), (128, 256, 128), (129, 264, 192), (333, 1720, 640), (700, 520, 1000),
-          (2048, 1024, 256)]
+          (2048, 1024, 256), (12400, 1024, 136), (6272, 2048, 384)]
 
 
 def slack(a, b):

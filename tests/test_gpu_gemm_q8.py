@@ -64,7 +64,7 @@ def near(got, want, bound, what):
 
 
 SHAPES = [(1, 8, 16), (1, 4096, 1024), (3, 136, 144), (16, 128, 128), (17, 1000, 2048), (64, 1024, 4096), (65, 72, 272), (128, 256, 128), (200, 264, 400), (777, 1000, 1904),
-          (2100, 1032, 1024), (300, 2304, 768)]
+          (2100, 1032, 1024), (300, 2304, 768), (4090, 4088, 400), (8190, 4088, 272)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)

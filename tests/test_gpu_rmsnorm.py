@@ -79,7 +79,7 @@ def check_codes(q, scales, v):
     near(q.double() * scale, v, v.abs() * (2.0 ** -4 + FP32) + scale * 2.0 ** -10, "codes")
 
 
-@pytest.mark.parametrize("rows,D", [(1, 8), (3, 1024), (5, 120), (33, 136), (64, 512), (17, 520), (130, 1000), (6, 2048), (5, 2056), (9, 8192), (4100, 768)])
+@pytest.mark.parametrize("rows,D", [(1, 8), (3, 1024), (5, 120), (33, 136), (64, 512), (17, 520), (130, 1000), (6, 2048), (5, 2056), (9, 8192), (4100, 768), (8500, 2048)])
 def test_forward(rows, D):
     x, residual, gamma = inputs(rows, D, rows * 8192 + D)
     total, y, q, scales = forward(x, residual, gamma)
@@ -154,7 +154,7 @@ def exact_backward(h, dy, gamma):
     return s * (t - h * pull), terms, (dy * h * s).sum(0), (dy * h * s).abs().sum(0)
 
 
-@pytest.mark.parametrize("rows,D", [(1, 8), (2, 1024), (7, 136), (65, 512), (130, 1000), (12, 2048), (11, 2056), (5, 8192), (6500, 768)])
+@pytest.mark.parametrize("rows,D", [(1, 8), (2, 1024), (7, 136), (65, 512), (130, 1000), (12, 2048), (11, 2056), (5, 8192), (6500, 768), (8500, 2048)])
 def test_backward(rows, D):
     h, residual, gamma = inputs(rows, D, rows * 8192 + D + 1)
     dy = torch.randn(rows, D, generator=torch.Generator().manual_seed(rows)).to(BF16).cuda()

@@ -24,8 +24,11 @@ GATED = dict(stream=None, M=4, F=64, D=32, X=A, ldx=32, W=A, ldw=32, H=A, ldh=64
 GATED_BACK = dict(stream=None, M=4, F=64, D=32, dY=A, lddy=32, Wdt=A, ldwdt=32, GU=A, ldgu=128, dGU=2 * A, lddgu=128, Wt=A, ldwt=128, dX=A, lddx=32, act=0)
 
 
+HUGE = (1 << 30) + 1
+
+
 @pytest.mark.parametrize("changes,needle", [
-    (dict(rows=0), b"rows"), (dict(D=0), b"multiple of 8"), (dict(D=12), b"multiple of 8"), (dict(D=8200), b"8192"), (dict(eps=-1.0), b"eps"),
+    (dict(rows=0), b"rows"), (dict(rows=HUGE, ld_scales=HUGE), b"rows"), (dict(D=0), b"multiple of 8"), (dict(D=12), b"multiple of 8"), (dict(D=8200), b"8192"), (dict(eps=-1.0), b"eps"),
     (dict(eps=float("nan")), b"eps"), (dict(eps=float("inf")), b"eps"), (dict(x=None), b"x"), (dict(x=A + 2), b"aligned"), (dict(hi=None), b"gamma_hi"),
     (dict(lo=A + 8), b"gamma_lo"), (dict(residual=A + 2), b"residual"), (dict(sum=None), b"sum"), (dict(y=None, q=None), b"no output"),
     (dict(y=A + 8), b"y"), (dict(q=A + 4), b"q"), (dict(scales=None), b"scales"), (dict(ld_scales=3), b"ld_scales")])
@@ -34,7 +37,7 @@ def test_norm(changes, needle):
 
 
 @pytest.mark.parametrize("changes,needle", [
-    (dict(rows=-1), b"rows"), (dict(D=20), b"multiple of 8"), (dict(dy=None), b"dy"), (dict(dx=A + 2), b"dx"), (dict(dgamma=None), b"dgamma"),
+    (dict(rows=-1), b"rows"), (dict(rows=HUGE), b"rows"), (dict(D=20), b"multiple of 8"), (dict(dy=None), b"dy"), (dict(dx=A + 2), b"dx"), (dict(dgamma=None), b"dgamma"),
     (dict(residual=A + 2), b"residual"), (dict(workspace=None), b"workspace"), (dict(workspace=A + 4), b"workspace"), (dict(size=64), b"workspace")])
 def test_norm_backward(changes, needle):
     refused(bridge.library().tgk_rmsnorm_bwd(*arguments(NORM_BACK, changes)), needle)
@@ -60,7 +63,7 @@ def test_weights(changes, needle):
 
 
 @pytest.mark.parametrize("changes,needle", [
-    (dict(M=0), b"M at least 1"), (dict(N=60), b"multiple of 8"), (dict(K=264), b"multiple of 16"), (dict(K=0), b"K"), (dict(X=None), b"X"),
+    (dict(M=0), b"M at least 1"), (dict(M=HUGE, ldxs=HUGE), b"at most"), (dict(N=1 << 30, ldy=1 << 30), b"Y"), (dict(N=60), b"multiple of 8"), (dict(K=264), b"multiple of 16"), (dict(K=0), b"K"), (dict(X=None), b"X"),
     (dict(X=A + 8), b"X"), (dict(ldx=264), b"X"), (dict(ldx=128), b"X"), (dict(W=A + 1), b"W"), (dict(ldw=1 << 23), b"W"), (dict(xs=None), b"x_scales"),
     (dict(ldxs=3), b"x_scales"), (dict(ws=A + 2), b"w_scales"), (dict(ldws=1), b"w_scales"), (dict(Y=None), b"Y"), (dict(ldy=60), b"Y"),
     (dict(residual=A + 2, ldr=64), b"residual"), (dict(residual=2 * A, ldr=32), b"residual"), (dict(residual=A, ldr=72), b"in place")])
@@ -69,7 +72,7 @@ def test_product(changes, needle):
 
 
 @pytest.mark.parametrize("changes,needle", [
-    (dict(M=0), b"M at least 1"), (dict(F=60), b"multiples of 8"), (dict(D=4), b"multiples of 8"), (dict(act=2), b"activation"), (dict(act=-1), b"activation"),
+    (dict(M=0), b"M at least 1"), (dict(M=HUGE), b"at most"), (dict(F=60), b"multiples of 8"), (dict(D=4), b"multiples of 8"), (dict(act=2), b"activation"), (dict(act=-1), b"activation"),
     (dict(X=None), b"X"), (dict(ldx=24), b"X"), (dict(W=A + 2), b"W"), (dict(ldw=36), b"W"), (dict(H=None), b"H"), (dict(ldh=32), b"H"), (dict(ldgu=64), b"GU"),
     (dict(ldx=1 << 22), b"X")])
 def test_gated(changes, needle):

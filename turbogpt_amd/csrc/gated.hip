@@ -171,8 +171,8 @@ void operand(const void *p, int ld, int columns, const char *what) {
         throw std::invalid_argument(std::string(what) + ": needs a 16-byte aligned pointer and a leading dimension that is a multiple of 8, at least the columns and at most 2^21");
 }
 void block_shape(int M, int F, int D, int activation, const char *where) {
-    if (M < 1 || F < 8 || D < 8 || F % 8 || D % 8 || F > MOST_LD / 2 || D > MOST_LD)
-        throw std::invalid_argument(std::string(where) + ": M at least 1, F and D multiples of 8 (F at most 2^20, D at most 2^21)");
+    if (M < 1 || M > MOST_ROWS || F < 8 || D < 8 || F % 8 || D % 8 || F > MOST_LD / 2 || D > MOST_LD)
+        throw std::invalid_argument(std::string(where) + ": M at least 1 and at most 2^30, F and D multiples of 8 (F at most 2^20, D at most 2^21)");
     if (activation != TGK_GATE_SILU && activation != TGK_GATE_GELU)
         throw std::invalid_argument(std::string(where) + ": activation is TGK_GATE_SILU or TGK_GATE_GELU");
 }
@@ -218,9 +218,10 @@ extern "C" int tgk_gated_bwd(hipStream_t stream, int M, int F, int D, const uint
         by_activation(activation, [&](auto act) { product_bf16<false>(stream, M, F, D, dY, lddy, Wdt, ldwdt, GatedBackward<act()>{GU, dGU, ldgu, lddgu}); });
         if (!dX)
             return;
-        // Widths that 192 divides and 256 does not leave a quarter of a 256-column tile empty: the framework's products have tiles of 192 (16384 x 768,
-        // 2F = 4096 91 us here, 82 there; x 1024, 2F = 8192 200 here, 218 there).
-        if (M % 128 == 0 && D % 192 == 0 && D % 256 != 0 && F % 64 == 0) {
+        // A plain product: the framework's, where it takes the shape.  With the product before it, us there and here: 16384 x 1024, F = 4096 366, 390; 8192 x 1024,
+        // F = 4096 208, 239; 8192 x 640, F = 2048 88, 97; 2048 x 256, F = 1024 17.4, 22.2.  Below 1024 rows the kernels here are as fast or faster (512 x 512,
+        // F = 2048 18.7, 18.2).
+        if (M % 128 == 0 && M >= 1024 && (D % 128 == 0 || D % 192 == 0) && F % 16 == 0) {
             if (tgk_gemm_dgrad_t(stream, M, 2 * F, D, dGU, lddgu, Wt, ldwt, dX, lddx, nullptr, 0) < 0)
                 throw std::runtime_error(tg_last_error);
             return;

@@ -370,7 +370,8 @@ void tile_kernel(Shape s, Epilogue epilogue) {
 }
 
 // A lane's offset into a tile is 32 bits wide: 256 rows of at most 2^22 bytes.
-constexpr int MOST_LD = 1 << 21; // elements of 16 bits
+constexpr int MOST_LD = 1 << 21;   // elements of 16 bits
+constexpr int MOST_ROWS = 1 << 30; // of either operand
 
 template <class T, class Epilogue> void launch_tiles(hipStream_t stream, Shape s, const Epilogue &epilogue) {
     s.tiles_m = (s.M + T::BM - 1) / T::BM, s.tiles_n = (s.N + T::COLUMNS - 1) / T::COLUMNS;

@@ -361,14 +361,14 @@ __global__ __launch_bounds__(256) void quantize_tiles_kernel(const bf16_t *__res
         scales[size_t(tile_row) * ld_scales + tile_column] = scale;
 }
 
-constexpr int MOST_D = 8192;
+constexpr int MOST_D = 8192, MOST_ROWS = 1 << 30;
 void pointer(const void *p, int alignment, const char *what) {
     if (!p || reinterpret_cast<uintptr_t>(p) & (alignment - 1))
         throw std::invalid_argument(std::string(what) + ": must be non-null and " + std::to_string(alignment) + "-byte aligned");
 }
 void norm_shape(int rows, int D, float eps, const char *where) {
-    if (rows < 1 || D < 8 || D % 8 || D > MOST_D || !(eps >= 0.f) || std::isinf(eps))
-        throw std::invalid_argument(std::string(where) + ": rows at least 1, D a multiple of 8 and at most 8192, eps finite and not negative");
+    if (rows < 1 || rows > MOST_ROWS || D < 8 || D % 8 || D > MOST_D || !(eps >= 0.f) || std::isinf(eps))
+        throw std::invalid_argument(std::string(where) + ": rows at least 1 and at most 2^30, D a multiple of 8 and at most 8192, eps finite and not negative");
 }
 int slots_of(int D) { return D <= 2048 ? 4 : 1; } // rows a block works on at a time
 // rows a block takes in all: one round of its slots, more where that would be more than 2048 blocks (16384 x 2048 to 8 bits 53 us with 1024, 50 with 2048)
@@ -427,7 +427,7 @@ extern "C" int tgk_rmsnorm_fwd(hipStream_t stream, int rows, int D, const uint16
 }
 
 extern "C" size_t tgk_rmsnorm_bwd_workspace(int rows, int D) {
-    return rows > 0 && D > 0 && D <= MOST_D ? size_t(backward_blocks(rows, D)) * D * sizeof(float) : 0;
+    return rows > 0 && rows <= MOST_ROWS && D > 0 && D <= MOST_D ? size_t(backward_blocks(rows, D)) * D * sizeof(float) : 0;
 }
 
 extern "C" int tgk_rmsnorm_bwd(hipStream_t stream, int rows, int D, const uint16_t *x, const uint16_t *dy, const uint16_t *gamma_hi, const uint16_t *gamma_lo,
