@@ -15,8 +15,19 @@
 namespace product {
 
 // WM x WN waves of (BM / WM) x 64 outputs.  AR and BR: slots of A's and B's rings; a stage is requested one less than that ahead.
-// PHASED: the two halves of the waves take turns (below), B's ring has two slots; otherwise both rings have as many.  GATED: B's rows are of two matrices on top of each other, N rows each; every wave's 64 are 32 of the upper
-// and the same 32 of the lower, and a tile has BN / 2 columns of the result.
+// GATED: B's rows are of two matrices on top of each other, N rows each; every wave's 64 are 32 of the upper and the same 32 of the lower, and a
+// tile has BN / 2 columns of the result.
+//
+// PHASED (256 x 256, eight waves, two on each SIMD, one of either half of the rows): a stage is cut into phases, in which a wave first reads its
+// fragments and requests copies and then multiplies, and the second half of the waves is one barrier behind the first, so that on every SIMD one wave
+// multiplies while the other reads.  Gated, 16384 rows, D = 768, F = 2048, pre-activations kept: tiles of 128 x 128 without phases 164 us, these 113 to 120; the
+// same tiles without phases 134 (8-bit ones do not keep their sums in registers so).  In bfloat16 two phases a stage, by halves of k (four: 5 %
+// slower), and three slots for A; in 8 bits four phases, by rows, as a matrix instruction takes the whole block of k.
+// What bounds them: bfloat16 runs at 1.8 to 1.9 GHz with the matrix pipe busy 65 to 70 % of the cycles, 1.6 us a stage with every unit at work; copies alone take
+// 1.1, all but the copies 1.2.  8 bits, at 2.1 GHz: 2.1 us; without scaling the products 1.8, without copies 1.55, without products 1.6, without
+// scaling and copies 1.2, so no one thing bounds it.  Tried there, all within 3 %: two phases; copies spread otherwise; both operands two stages ahead, into the
+// half of a slot that its phase has left; scaling put off to the next phase; no phases, one barrier a stage, fragments a row ahead.  In bfloat16: three slots for
+// A or two, copies before or behind the reads, both operands in the first phase, units started in turn so that their epilogues do not meet: nothing or slower.
 template <bool E4M3_, bool GATED_, int BM_, int BN_, int WM_, int WN_, int AR_, bool PHASED_ = false> struct Tile {
     static constexpr int BR = PHASED_ ? 2 : AR_;
     static constexpr bool E4M3 = E4M3_, GATED = GATED_, PHASED = PHASED_;
@@ -173,6 +184,8 @@ void tile_kernel(Shape s, Epilogue epilogue) {
         request_a();
     }
     const int tail = (s.k_bytes % STAGE + 15) >> 4; // chunks of the last stage, 0: all
+    // The wave's copies of the next stage are there.  In phases the first half of the waves asks behind its last products, the second in front of them: that
+    // is the same turn, the one before the first half reads that stage.
     const auto landed = [&](bool is_tail, int slot_a, int slot_b) {
         wait_vmcnt<(T::AR - 2) * (T::A_COPIES + T::SCALE_COPIES + (T::PHASED ? 0 : T::B_COPIES))>();
         if (is_tail) {
@@ -208,9 +221,9 @@ void tile_kernel(Shape s, Epilogue epilogue) {
 #pragma unroll
             for (int j = 0; j < T::FN; ++j)
                 acc[i][j] = f32x4{0, 0, 0, 0};
-        constexpr int PHASES = 4, ROWS = T::FM / PHASES ? T::FM / PHASES : 1; // 8-bit: fragment rows of a phase
+        constexpr int PHASES = 4, ROWS = T::FM / PHASES ? T::FM / PHASES : 1; // 8-bit: phases, and fragment rows of each
         if (T::PHASED && wm == 1)
-            turn();
+            turn(); // from here to the end of the tile one turn behind the other half
         for (int stage = 0; stage < s.stages; ++stage) {
             const uint32_t a_at = at + slot_a * T::A_BYTES + wm * (T::FM * 16 * STAGE) + lane_at;
             const uint32_t b_at = at + T::B_AT + slot_b * T::B_BYTES + wn * (T::FN * 16 * STAGE) + lane_at;
