@@ -208,7 +208,7 @@ TGK_API int tgk_layernorm_bwd_fold(hipStream_t stream, int rows, int D, int coun
 
 /* h = RN_bf16(x + residual) into `sum` (may be x or residual itself); residual NULL: h = x, `sum` is not used.
  * v = h * gamma / sqrt(mean(h^2) + eps) in fp32: RN_bf16(v) into y and / or codes into q and scales into `scales`; what is NULL is left out.
- * x, residual, sum, y, q are [rows][D], D a multiple of 8, at most 8192; 16-byte aligned, q 8-byte. */
+ * x, residual, sum, y, q are [rows][D], rows at most 2^30, D a multiple of 8, at most 8192; 16-byte aligned, q 8-byte. */
 TGK_API int tgk_rmsnorm_fwd(hipStream_t stream, int rows, int D, const uint16_t *x, const uint16_t *residual, const uint16_t *gamma_hi,
                             const uint16_t *gamma_lo, uint16_t *sum, uint16_t *y, uint8_t *q, float *scales, int ld_scales, float eps);
 /* x is what was normalised (the forward's sum).  dx = RN(residual + dv), dv the gradient through the norm in fp32, or RN(dv) where
@@ -228,15 +228,16 @@ TGK_API int tgk_quantize_tiles(hipStream_t stream, int rows, int columns, const 
 
 /* The linear layer on such operands, beside tgk_gemm_fwd:
  *   Y[m][n] = RN_bf16( sum_b x_scales[b][m] * w_scales[n / 128][b] * (sum over k in block b of X[m][k] W[n][k]) (+ residual[m][n]) )
- * products and sums in fp32, rounded once.  Any M; N a multiple of 8, K of 16; ldx and ldw multiples of 16, ldy and ldr of 8; scales
- * 4-byte, everything else 16-byte aligned.  The residual may be Y itself. */
+ * products and sums in fp32, rounded once.  Any M; N a multiple of 8, K of 16; ldx and ldw multiples of 16, ldy and ldr of 8 (M and N at
+ * most 2^30, K and leading dimensions 2^22); scales 4-byte, everything else 16-byte aligned.  The residual may be Y itself. */
 TGK_API int tgk_gemm_q8(hipStream_t stream, int M, int N, int K, const uint8_t *X, int ldx, const float *x_scales, int ldxs, const uint8_t *W,
                         int ldw, const float *w_scales, int ldws, uint16_t *Y, int ldy, const uint16_t *residual, int ldr);
 
 /* ---- Gated feed-forward block (swiglu_activation and swiglu_backward, cuda/ops.cuh:120-144, at any width, with the projections).
  * W[2F][D] holds the gate's rows and below them the up projection's (model.h:27-31).
  *   [G U] = X W^T,  H = RN_bf16(act(G) U) from the fp32 sums;  GU[M][2F] = RN_bf16 of both, for the backward pass (NULL: not written)
- * Any M, F and D multiples of 8; pointers 16-byte aligned, leading dimensions multiples of 8. ---- */
+ * Any M (at most 2^30), F and D multiples of 8 (at most 2^20 and 2^21); pointers 16-byte aligned, leading dimensions multiples of 8, at
+ * most 2^21. ---- */
 enum { TGK_GATE_SILU = 0, TGK_GATE_GELU = 1 /* exact erf */ };
 TGK_API int tgk_gated_fwd(hipStream_t stream, int M, int F, int D, const uint16_t *X, int ldx, const uint16_t *W, int ldw, uint16_t *H, int ldh,
                           uint16_t *GU, int ldgu, int activation);

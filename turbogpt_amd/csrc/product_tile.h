@@ -23,10 +23,11 @@ namespace product {
 // multiplies while the other reads.  Gated, 16384 rows, D = 768, F = 2048, pre-activations kept: tiles of 128 x 128 without phases 164 us, these 113 to 120; the
 // same tiles without phases 134 (8-bit ones do not keep their sums in registers so).  In bfloat16 two phases a stage, by halves of k (four: 5 %
 // slower), and three slots for A; in 8 bits four phases, by rows, as a matrix instruction takes the whole block of k.
-// What bounds them: bfloat16 runs at 1.8 to 1.9 GHz with the matrix pipe busy 65 to 70 % of the cycles, 1.6 us a stage with every unit at work; copies alone take
+// What bounds them: bfloat16 runs at 1.8 to 1.9 GHz with the matrix pipe busy 65 to 70 % of the cycles (8192 k), 1.6 us a stage with every unit at work; copies alone take
 // 1.1, all but the copies 1.2.  8 bits, at 2.1 GHz: 2.1 us; without scaling the products 1.8, without copies 1.55, without products 1.6, without
 // scaling and copies 1.2, so no one thing bounds it.  Tried there, all within 3 %: two phases; copies spread otherwise; both operands two stages ahead, into the
-// half of a slot that its phase has left; scaling put off to the next phase; no phases, one barrier a stage, fragments a row ahead.  In bfloat16: three slots for
+// half of a slot that its phase has left; scaling put off to the next phase; no phases, one barrier a stage, fragments a row ahead.  Instructions of
+// 32 x 32 results: 5 to 8 % slower.  In bfloat16: three slots for
 // A or two, copies before or behind the reads, both operands in the first phase, units started in turn so that their epilogues do not meet: nothing or slower.
 template <bool E4M3_, bool GATED_, int BM_, int BN_, int WM_, int WN_, int AR_, bool PHASED_ = false> struct Tile {
     static constexpr int BR = PHASED_ ? 2 : AR_;
