@@ -11,7 +11,8 @@ A case is a dict of plain values with a "kind":
               scale for each 128 x 128 tile, and the residual
 
 Rows are tokens, D is the model's width, F the block's hidden width.  prepare() makes a case's inputs from the seed and what a
-program keeps (weights, their transposed copies, buffers); run() is one pass.
+program keeps (weights, buffers, the down projection's transposed copy, which both sides read); run() is one pass.  The packed weight's
+transposed copy, which only the framework's backward pass reads, is made in the pass: the weights change with every step.
 """
 import math
 
@@ -230,6 +231,20 @@ def _plain(s):
     return dict(y=y.to(BF16)) if s["rows8"] else dict(y=y.to(BF16), q=q, scales=scales)
 
 
+def _transpose(s, lib, stream):
+    """The packed weight's transposed copy, by the framework's entry where it takes the shape."""
+    w, w_t = s["w"], s["w_t"]
+    rows, columns = w.shape
+    if rows % 64 or columns % 64:
+        w_t.copy_(w.t())
+        return
+    tiles = rows // 64 * (columns // 64)
+    if "transpose" not in s:  # one matrix: {int64 offset; int32 rows, columns, first tile, 0}
+        s["transpose"] = torch.tensor([0, rows | columns << 32, 0], device="cuda")
+    from turbogpt_amd.bridge import check
+    check(lib.tgk_transpose_batch(stream, w.data_ptr(), w_t.data_ptr(), s["transpose"].data_ptr(), 1, tiles))
+
+
 def _own(s):
     from turbogpt_amd.bridge import check, library
     lib, kind, m = library(), s["kind"], s["m"]
@@ -255,6 +270,7 @@ def _own(s):
                                 s["gu"].data_ptr() if train else None, 2 * f, act))
         if not train:
             return dict(h=s["h"])
+        _transpose(s, lib, stream)  # the weights are new in every step
         check(lib.tgk_gated_bwd(stream, m, f, d, s["dy"].data_ptr(), d, s["down_t"].data_ptr(), d, s["gu"].data_ptr(), 2 * f,
                                 s["dgu"].data_ptr(), 2 * f, s["w_t"].data_ptr(), 2 * f, s["dx"].data_ptr(), d, act))
         return dict(h=s["h"], gu=s["gu"], dgu=s["dgu"], dx=s["dx"])
