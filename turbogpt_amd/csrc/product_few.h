@@ -24,11 +24,8 @@ template <bool E4M3_, bool GATED_, int MT_, int NT_, int RING_> struct Few {
 template <class T, class Epilogue> __global__ __launch_bounds__(FEW_WAVES * 64, 2) void few_kernel(Shape s, Epilogue epilogue) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // blocks of the same columns are eight apart, in one XCD, which has their rows of b in its L2
-    const int group = blockIdx.x >> 3, tn = group / s.tiles_m * 8 + (blockIdx.x & 7), tm = group % s.tiles_m;
-    if (tn >= s.tiles_n)
-        return;
-    const int m0 = tm * T::MT * 16, n0 = tn * T::NT * 16, row = lane & 15;
+    const Place place = few_place(blockIdx.x, s.tiles_m, s.tiles_n);
+    const int m0 = place.m * T::MT * 16, n0 = place.n * T::NT * 16, row = lane & 15;
     const uint32_t ring = lds_address(lds) + wave * (T::RING * T::SLOT_BYTES);
     const int chunk = (lane & 7) ^ (lane >> 3);
     uint32_t a_offset[T::A_COPIES], b_offset[2 * T::NT];
@@ -184,11 +181,10 @@ template <class Kernel> void allow_lds(Kernel kernel, std::atomic<uint64_t> &con
 template <class T, class Epilogue> void launch_few(hipStream_t stream, Shape s, const Epilogue &epilogue) {
     s.tiles_m = (s.M + T::MT * 16 - 1) / (T::MT * 16), s.tiles_n = (s.N + T::NT * 16 - 1) / (T::NT * 16);
     s.stages = (s.k_bytes + STAGE - 1) / STAGE;
-    const int64_t blocks = int64_t((s.tiles_n + 7) / 8 * 8) * s.tiles_m;
-    require(blocks < (int64_t(1) << 30), "product: too many tiles");
+    s.tiles = s.tiles_m * s.tiles_n; // at most 256, launch_product
     static std::atomic<uint64_t> configured;
     allow_lds(few_kernel<T, Epilogue>, configured, T::LDS_BYTES);
-    hipLaunchKernelGGL((few_kernel<T, Epilogue>), dim3(int(blocks)), dim3(FEW_WAVES * 64), T::LDS_BYTES, stream, s, epilogue);
+    hipLaunchKernelGGL((few_kernel<T, Epilogue>), dim3(s.tiles), dim3(FEW_WAVES * 64), T::LDS_BYTES, stream, s, epilogue);
     check_hip(hipGetLastError(), "product launch: ");
 }
 

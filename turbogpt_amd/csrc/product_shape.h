@@ -1,6 +1,7 @@
 // What the products of product_tile.h and product_few.h work on.
 #pragma once
 #include "common.h"
+#include "product_launch.h"
 #include <atomic>
 #include <type_traits>
 

@@ -149,13 +149,6 @@ TG_DEVICE void pin(f32x4 &v) {
     asm volatile("" : "+v"(v));
 }
 
-// Tiles in the order in which a block meets them: a block's neighbours in its XCD (blocks 8 apart) take neighbouring tiles,
-// which share rows of a and b in that XCD's L2.
-TG_DEVICE int first_tile(int block, int grid) {
-    const int each = grid >> 3, rest = grid & 7, xcd = block & 7;
-    return xcd * each + (xcd < rest ? xcd : rest) + (block >> 3);
-}
-
 template <class T, class Epilogue> __global__ __launch_bounds__(T::THREADS, T::LDS_BYTES > 81920 ? T::WAVES / 4 : T::WAVES / 2)
 void tile_kernel(Shape s, Epilogue epilogue) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
