@@ -76,8 +76,8 @@ void scales(const float *p, int ld, int columns, const char *what) {
 extern "C" int tgk_gemm_q8(hipStream_t stream, int M, int N, int K, const uint8_t *X, int ldx, const float *x_scales, int ldxs, const uint8_t *W, int ldw,
                            const float *w_scales, int ldws, uint16_t *Y, int ldy, const uint16_t *residual, int ldr) {
     return guarded([&] {
-        require(M > 0 && N > 0 && K > 0 && N % 8 == 0 && K % 16 == 0 && M <= MOST_ROWS && N <= MOST_ROWS && K <= 2 * MOST_LD,
-                "gemm_q8: M at least 1, N a multiple of 8 (both at most 2^30), K a multiple of 16 (at most 2^22)");
+        require(M > 0 && N > 0 && K > 0 && N % 8 == 0 && K % 16 == 0 && M <= MOST_ROWS && N <= 2 * MOST_LD && K <= 2 * MOST_LD,
+                "gemm_q8: M at least 1 and at most 2^30, N a multiple of 8 and at most 2^22 (as Y's leading dimension), K a multiple of 16 and at most 2^22");
         operand(X, ldx, K, 16, "gemm_q8: X");
         operand(W, ldw, K, 16, "gemm_q8: W");
         operand(Y, ldy, N, 8, "gemm_q8: Y");
