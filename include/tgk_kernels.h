@@ -219,10 +219,11 @@ TGK_API int tgk_rmsnorm_bwd(hipStream_t stream, int rows, int D, const uint16_t 
                             void *workspace, size_t workspace_bytes);
 TGK_API size_t tgk_rmsnorm_bwd_workspace(int rows, int D);
 
-/* bf16 rows [rows][ldx] into codes [rows][ldq] and scales as above.  columns and both leading dimensions multiples of 8. */
+/* bf16 rows [rows][ldx] into codes [rows][ldq] and scales as above.  columns and both leading dimensions multiples of 8; fewer than
+ * 2^24 blocks of 32 rows and 512 columns. */
 TGK_API int tgk_quantize_rows(hipStream_t stream, int rows, int columns, const uint16_t *x, int ldx, uint8_t *q, int ldq, float *scales,
                               int ld_scales);
-/* A weight: one scale for each tile of 128 x 128, scales [ceil(rows / 128)][ld_scales], ld_scales >= ceil(columns / 128). */
+/* A weight: one scale for each tile of 128 x 128, scales [ceil(rows / 128)][ld_scales], ld_scales >= ceil(columns / 128); fewer than 2^24 tiles. */
 TGK_API int tgk_quantize_tiles(hipStream_t stream, int rows, int columns, const uint16_t *w, int ldw, uint8_t *q, int ldq, float *scales,
                                int ld_scales);
 

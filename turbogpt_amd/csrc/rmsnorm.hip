@@ -363,7 +363,7 @@ __global__ __launch_bounds__(256) void quantize_tiles_kernel(const bf16_t *__res
         scales[size_t(tile_row) * ld_scales + tile_column] = scale;
 }
 
-constexpr int MOST_D = 8192, MOST_ROWS = 1 << 30;
+constexpr int MOST_D = 8192, MOST_ROWS = 1 << 30, MOST_BLOCKS = 1 << 24; // blocks: of 256 work items, of which a launch holds fewer than 2^32
 void pointer(const void *p, int alignment, const char *what) {
     if (!p || reinterpret_cast<uintptr_t>(p) & (alignment - 1))
         throw std::invalid_argument(std::string(what) + ": must be non-null and " + std::to_string(alignment) + "-byte aligned");
@@ -467,7 +467,7 @@ extern "C" int tgk_quantize_rows(hipStream_t stream, int rows, int columns, cons
         require(ld_scales >= rows, "quantize_rows: ld_scales must be at least the rows");
         const int parts = (columns - 1) / 512 + 1;
         const int64_t blocks = int64_t((rows - 1) / QUANTIZE_ROWS + 1) * parts;
-        require(blocks < (int64_t(1) << 30), "quantize_rows: too many rows and columns");
+        require(blocks < MOST_BLOCKS, "quantize_rows: too many rows and columns: 2^24 blocks of 32 rows and 512 columns or more");
         hipLaunchKernelGGL(quantize_rows_kernel, dim3(int(blocks)), dim3(256), 0, stream, x, ldx, q, ldq, scales, ld_scales, rows, columns, parts);
         check_hip(hipGetLastError(), "quantize_rows launch: ");
     });
@@ -482,7 +482,7 @@ extern "C" int tgk_quantize_tiles(hipStream_t stream, int rows, int columns, con
         require(ldw >= columns && ldw % 8 == 0 && ldq >= columns && ldq % 8 == 0, "quantize_tiles: leading dimensions must be multiples of 8, at least the columns");
         const int tiles_m = (rows - 1) / 128 + 1, tiles_n = (columns - 1) / 128 + 1;
         require(ld_scales >= tiles_n, "quantize_tiles: ld_scales must be at least the tiles of a row");
-        require(int64_t(tiles_m) * tiles_n < (int64_t(1) << 30), "quantize_tiles: too many tiles");
+        require(int64_t(tiles_m) * tiles_n < MOST_BLOCKS, "quantize_tiles: too many tiles: 2^24 blocks of 128 x 128 or more");
         hipLaunchKernelGGL(quantize_tiles_kernel, dim3(tiles_m * tiles_n), dim3(256), 0, stream, w, ldw, q, ldq, scales, ld_scales, rows, columns, tiles_n);
         check_hip(hipGetLastError(), "quantize_tiles launch: ");
     });
