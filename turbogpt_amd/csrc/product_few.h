@@ -18,7 +18,7 @@ template <bool E4M3_, bool GATED_, int MT_, int NT_, int RING_> struct Few {
     static constexpr int A_COPIES = 2 * MT, B_COPIES = 2 * NT * MATRICES, COPIES = A_COPIES + B_COPIES + (E4M3 ? 2 : 0);
     static constexpr int SCALES_AT = (A_COPIES + B_COPIES) * 1024, SLOT_BYTES = SCALES_AT + (E4M3 ? 512 : 0); // 64 floats of rows, 64 of columns
     static constexpr int RINGS = FEW_WAVES * RING * SLOT_BYTES, MEET = FEW_WAVES * TILES * 1024, LDS_BYTES = RINGS > MEET ? RINGS : MEET;
-    static_assert(RING <= 4 && LDS_BYTES <= 163840, "few");
+    static_assert((RING == 1 || RING == 2) && LDS_BYTES <= 163840, "few");
 };
 
 template <class T, class Epilogue> __global__ __launch_bounds__(FEW_WAVES * 64, 2) void few_kernel(Shape s, Epilogue epilogue) {
@@ -78,15 +78,11 @@ template <class T, class Epilogue> __global__ __launch_bounds__(FEW_WAVES * 64, 
             request(wave + r * FEW_WAVES, r);
     int slot = 0;
     for (int i = 0; i < count; ++i) {
-        const int stage = wave + i * FEW_WAVES, behind = count - 1 - i < T::RING - 1 ? count - 1 - i : T::RING - 1; // stages requested since
-        if (behind == 0)
-            wait_vmcnt<0>();
-        else if (behind == 1)
+        const int stage = wave + i * FEW_WAVES;
+        if (T::RING == 2 && i + 1 < count) // the next stage has been requested since
             wait_vmcnt<T::COPIES>();
-        else if (behind == 2)
-            wait_vmcnt<2 * T::COPIES>();
         else
-            wait_vmcnt<3 * T::COPIES>();
+            wait_vmcnt<0>();
         const uint32_t at = ring + slot * T::SLOT_BYTES;
         if (stage + 1 == s.stages && chunk >= last_chunks) { // zeros in both operands: what lies behind a row's end may be anything
 #pragma unroll
