@@ -384,50 +384,32 @@ template <class T, class Epilogue> void launch_tiles(hipStream_t stream, Shape s
     s.tiles_m = (s.M + T::BM - 1) / T::BM, s.tiles_n = (s.N + T::COLUMNS - 1) / T::COLUMNS;
     require(int64_t(s.tiles_m) * s.tiles_n < (int64_t(1) << 30), "product: too many tiles");
     s.tiles = s.tiles_m * s.tiles_n, s.stages = (s.k_bytes + STAGE - 1) / STAGE;
-    const int most = T::LDS_BYTES > 81920 ? 256 : 512;
+    constexpr int most = most_blocks(T::BM == 256 ? TILES_256 : TILES_128);
+    static_assert(most == (T::LDS_BYTES > 81920 ? 256 : 512), "tiles: blocks of a unit");
     static std::atomic<uint64_t> configured;
     allow_lds(tile_kernel<T, Epilogue>, configured, T::LDS_BYTES);
     hipLaunchKernelGGL((tile_kernel<T, Epilogue>), dim3(s.tiles < most ? s.tiles : most), dim3(T::THREADS), T::LDS_BYTES, stream, s, epilogue);
     check_hip(hipGetLastError(), "product launch: ");
 }
-// Which kernel.  While 256 blocks, one a unit, cover the result, the smallest of the few kernel's shapes that does it (its blocks share out k, so one
-// is never worse than more: 1000 columns, K = 1904 in 8 bits, 1024 rows 11.3 us, tiles of 64 x 128 14.3; at 2048 rows, 512 blocks, 18 and 15.2).
-// Otherwise the least of the tiles' estimated times, us: per stage a tile's time alone on its unit, or of two (of 256 x 256 it grows with the
-// share of units that have one, as all of them ask the same memory), and an epilogue; fitted to the operators at 64 to 16384 rows.  Gated, 2 x 2816
-// columns, D = 1024, on 64 x 128, 128 x 128, 256 x 256: 512 rows 15.8, 17.7, 26; 1024 28.9, 20.7, 27.5; 2048 40, 40, 30.
-struct TileTimes {
-    double alone, two, epilogue;
-};
-inline double tiles_us(int64_t tiles, int stages, const TileTimes &t) {
-    const int64_t rounds = tiles / 512, rest = tiles % 512;
-    return rounds * (stages * t.two + t.epilogue) + (rest > 256 ? stages * t.two + t.epilogue : rest ? stages * t.alone + t.epilogue : 0.0);
-}
-inline double large_tiles_us(int64_t tiles, int stages, const TileTimes &t) { // `two`: alone, with every unit at work
-    const int64_t rounds = tiles / 256, rest = tiles % 256;
-    return rounds * (stages * t.two + t.epilogue) + (rest ? stages * (t.alone + (t.two - t.alone) * (rounds ? 1.0 : rest / 256.0)) + t.epilogue : 0.0);
-}
 template <bool E4M3, bool GATED, class Epilogue> void launch_product(hipStream_t stream, Shape s, const Epilogue &epilogue) {
-    s.stages = (s.k_bytes + STAGE - 1) / STAGE;
-    const auto count = [&](int rows, int columns) { return int64_t((s.M + rows - 1) / rows) * ((s.N + columns - 1) / columns); };
-    if (count(16, 16) <= 256)
+    switch (product_kernel(s.M, s.N, (s.k_bytes + STAGE - 1) / STAGE, E4M3, GATED)) {
+    case FEW_16:
         return launch_few<Few<E4M3, GATED, 1, 1, 2>>(stream, s, epilogue);
-    if (count(32, 32) <= 256)
+    case FEW_32:
         return launch_few<Few<E4M3, GATED, 2, 2, 1>>(stream, s, epilogue);
-    if (count(64, 32) <= 256)
+    case FEW_64x32:
         return launch_few<Few<E4M3, GATED, 4, 2, 1>>(stream, s, epilogue);
-    if constexpr (!GATED)
-        if (count(64, 64) <= 256)
+    case FEW_64:
+        if constexpr (!GATED)
             return launch_few<Few<E4M3, GATED, 4, 4, 1>>(stream, s, epilogue);
-    constexpr int OF = GATED ? 2 : 1; // a tile's columns of B for one of the result
-    const double low = tiles_us(count(64, 128 / OF), s.stages, E4M3 ? TileTimes{0.54, 0.90, 1.5} : TileTimes{0.42, 0.72, 1.5});
-    const double square = tiles_us(count(128, 128 / OF), s.stages, E4M3 ? TileTimes{0.77, 1.25, 2.5} : TileTimes{0.57, 1.10, 2.5});
-    const double large = large_tiles_us(count(256, 256 / OF), s.stages, E4M3 ? TileTimes{1.65, 1.90, 6.0} : TileTimes{0.95, 1.58, 6.0});
-    if (large <= low && large <= square)
-        launch_tiles<Tile<E4M3, GATED, 256, 256, 2, 4, E4M3 ? 2 : 3, true>>(stream, s, epilogue);
-    else if (square <= low)
-        launch_tiles<Tile<E4M3, GATED, 128, 128, 2, 2, 2>>(stream, s, epilogue);
-    else
-        launch_tiles<Tile<E4M3, GATED, 64, 128, 2, 2, 3>>(stream, s, epilogue);
+        break;
+    case TILES_64x128:
+        return launch_tiles<Tile<E4M3, GATED, 64, 128, 2, 2, 3>>(stream, s, epilogue);
+    case TILES_128:
+        return launch_tiles<Tile<E4M3, GATED, 128, 128, 2, 2, 2>>(stream, s, epilogue);
+    case TILES_256:
+        return launch_tiles<Tile<E4M3, GATED, 256, 256, 2, 4, E4M3 ? 2 : 3, true>>(stream, s, epilogue);
+    }
 }
 
 } // namespace product
