@@ -208,7 +208,8 @@ TGK_API int tgk_layernorm_bwd_fold(hipStream_t stream, int rows, int D, int coun
 
 /* h = RN_bf16(x + residual) into `sum` (may be x or residual itself); residual NULL: h = x, `sum` is not used.
  * v = h * gamma / sqrt(mean(h^2) + eps) in fp32: RN_bf16(v) into y and / or codes into q and scales into `scales`; what is NULL is left out.
- * x, residual, sum, y, q are [rows][D], rows at most 2^30, D a multiple of 8, at most 8192; 16-byte aligned, q 8-byte. */
+ * x, residual, sum, y, q are [rows][D], rows at most 2^30, D a multiple of 8, at most 8192; 16-byte aligned, q 8-byte (where
+ * tgk_gemm_q8 reads the codes, D a multiple of 16 and q 16-byte aligned). */
 TGK_API int tgk_rmsnorm_fwd(hipStream_t stream, int rows, int D, const uint16_t *x, const uint16_t *residual, const uint16_t *gamma_hi,
                             const uint16_t *gamma_lo, uint16_t *sum, uint16_t *y, uint8_t *q, float *scales, int ld_scales, float eps);
 /* x is what was normalised (the forward's sum).  dx = RN(residual + dv), dv the gradient through the norm in fp32, or RN(dv) where
@@ -242,12 +243,13 @@ TGK_API int tgk_gemm_q8(hipStream_t stream, int M, int N, int K, const uint8_t *
  * W[2F][D] holds the gate's rows and below them the up projection's (model.h:27-31).
  *   [G U] = X W^T,  H = RN_bf16(act(G) U) from the fp32 sums;  GU[M][2F] = RN_bf16 of both, for the backward pass (NULL: not written)
  * Any M (at most 2^30), F and D multiples of 8 (at most 2^20 and 2^21); pointers 16-byte aligned, leading dimensions multiples of 8, at
- * most 2^21. ---- */
+ * most 2^21.  These are the gated entries' own limits: tgk_gemm_fwd, tgk_gemm_wgrad and tgk_transpose_batch, which the rest of the block goes through, ask for
+ * the multiples named there. ---- */
 enum { TGK_GATE_SILU = 0, TGK_GATE_GELU = 1 /* exact erf */ };
 TGK_API int tgk_gated_fwd(hipStream_t stream, int M, int F, int D, const uint16_t *X, int ldx, const uint16_t *W, int ldw, uint16_t *H, int ldh,
                           uint16_t *GU, int ldgu, int activation);
-/* Backward from dY, the gradient of the block's output Y = H Wd^T (Wd[D][F], tgk_gemm_fwd), with the transposed copies of the
- * weights (tgk_transpose_batch), Wdt[F][D] and Wt[D][2F]:
+/* Backward from dY, the gradient of the block's output Y = H Wd^T (Wd[D][F], tgk_gemm_fwd), with transposed copies of the
+ * weights (tgk_transpose_batch, or any other copy where 64 does not divide the sizes), Wdt[F][D] and Wt[D][2F]:
  *   dH = dY Wd (not written),  dGU = [RN(dH U act'(G))  RN(dH act(G))],  dX = RN(dGU W); dX NULL: not computed, Wt not read.
  * dGU may be GU itself.  The weights' gradients are tgk_gemm_wgrad products: dW[2F][D] = dGU^T X and dWd = dY^T H. */
 TGK_API int tgk_gated_bwd(hipStream_t stream, int M, int F, int D, const uint16_t *dY, int lddy, const uint16_t *Wdt, int ldwdt, const uint16_t *GU,
