@@ -7,9 +7,11 @@
 // pre-activations and writes dG = dH u act'(g) and dU = dH act(g); dH itself never reaches memory.  dX = [dG dU] W is a plain
 // product over 2F.
 //
-// Measured, us: 16384 x 768, F = 2048 forward with both pre-activations kept 105 to 120 (103 GFLOP, 0.29 GB), dH's product 80 to 88 (51 GFLOP, 0.33 GB); 16384 x 1024, F = 4096 246 to 271
-// and 182 to 193 (275 and 137 GFLOP).  dH's epilogue reads and writes four values for each sum: its memory traffic alone takes 112 us of the 182, the products alone
-// 100, and as every unit comes to it with the clock and the L2s shared they add up.  One token, 1024 -> 2816: 3.9, 11.5 MB of weights.
+// Measured, us, least and median of thirty launches with others between them: 16384 x 768, F = 2048 forward with both pre-activations kept 106 and 125 (103 GFLOP,
+// 0.23 GB of operands and results, of which 0.202 are written, as counted, and 0.201 have to be), dH's product 81 and 91 (51 GFLOP, 0.30 GB); 16384 x 1024,
+// F = 4096, GELU 254 and 270, and 187 and 195 (275 and 137 GFLOP).  dH's epilogue reads and writes four values for each sum: its memory traffic alone takes
+// 112 us of the 187, the products alone 100, and as every unit comes to it with the clock and the L2s shared they add up.  One token, 1024 -> 2816: 3.9,
+// 11.5 MB of weights.
 //
 // The weights' gradients are dW = [dG dU]^T X and dWd = dY^T H: tgk_gemm_wgrad.
 #include "product_tile.h"

@@ -8,8 +8,9 @@
 // The product of the scales leaves fp32's normal range for values that are below 2^-60 on both sides, say; scaling by one after the other would not, but takes
 // another multiplication for each sum: 16384 x 4096, K = 4096 302 us -> 349.  With the powers of two given to the matrix instruction 329; with a branch, by
 // wave, to the slower form 407.
-// Measured: 16384 x 4096, K = 4096 260 us (2.1 PFLOP/s; with a residual 290 to 310), a vendor library's product with one scale an operand 217; 64 x 1024, K = 4096 4.6,
-// one token, 1024 -> 4096 3.4 (4.2 MB of weights).  What bounds the large one: product_tile.h.  No counterpart in the reference; it stands beside tgk_gemm_fwd (project, cuda/mma.cuh:77-108).
+//
+// Measured, over machines: 16384 x 4096, K = 4096 280 to 310 us (1.8 to 2.0 PFLOP/s; with a residual 295 to 310, behind the rows' quantisation 318 to 336), a vendor
+// library's product with one scale an operand 217; 64 x 1024, K = 4096 4.5, one token, 1024 -> 4096 3.2 (4.2 MB of weights).  What bounds the large one: product_tile.h.  No counterpart in the reference; it stands beside tgk_gemm_fwd (project, cuda/mma.cuh:77-108).
 #include "product_tile.h"
 #include "../../include/tgk_kernels.h"
 

@@ -24,7 +24,8 @@ constexpr Place few_place(int block, int tiles_m, int tiles_n) {
 // Which kernel.  While 256 blocks, one a unit, cover the result, the smallest of the few kernel's shapes that does it (its blocks share out k, so one
 // is never worse than more: 1000 columns, K = 1904 in 8 bits, 1024 rows 11.3 us, tiles of 64 x 128 14.3; at 2048 rows, 512 blocks, 18 and 15.2).
 // Otherwise the least of the tiles' estimated times, us: per stage a tile's time alone on its unit, or of two (of 256 x 256 it grows with the
-// share of units that have one, as all of them ask the same memory), and an epilogue; fitted to the operators at 64 to 16384 rows.  Gated, 2 x 2816
+// share of units that have one, as all of them ask the same memory), and an epilogue; fitted to the operators at 64 to 16384 rows, by what they choose: a
+// pass by itself may take longer (gated, 333 rows, 1720 columns, D = 640 on 64 x 128: 8.4, estimated 5.7).  Gated, 2 x 2816
 // columns, D = 1024, on 64 x 128, 128 x 128, 256 x 256: 512 rows 15.8, 17.7, 26; 1024 28.9, 20.7, 27.5; 2048 40, 40, 30.
 enum ProductKernel { FEW_16, FEW_32, FEW_64x32, FEW_64, TILES_64x128, TILES_128, TILES_256 };
 // how many blocks of a kernel of tiles are at work at a time, on 256 units

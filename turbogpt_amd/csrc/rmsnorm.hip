@@ -7,8 +7,9 @@
 //   dx = RN(residual gradient + s gamma dy - h s^3 mean(h gamma dy)), dgamma = sum over rows of dy h s
 //
 // All of them are bound by memory: a row is read once, held in registers while its sum of squares is taken, and written, and the next row is on its way
-// meanwhile.  Where a copy of 1 GiB reaches 5.0 TB/s: 16384 x 2048 with the sum and 8-bit output 45.5 us (5.2 TB/s), 16384 x 768 forward 18.2 (5.5), backward 20 (5.0)
-// + 4 for the fold of dgamma; rows to codes 16384 x 4096 36 to 42 (4.8 to 5.6).  One row: 2.3 us.
+// meanwhile.  Where a copy of 1 GiB reaches 5.0 TB/s, medians of thirty launches: 16384 x 2048 with the sum and 8-bit output 45.5 us (5.2 TB/s), without a residual
+// to bfloat16 24 (5.6); 16384 x 768 forward 19.6 (5.1), backward 20.2 (5.0) + 4.6 for the fold of dgamma; 4096 x 8192 forward 44.6 (6.0), backward with the fold 67.6
+// (4.0); 16384 x 4096 backward 106 (5.0).  Rows to codes 16384 x 4096 36 to 42 (4.8 to 5.6), a weight of 4096 x 4096 12.3 (4.1).  One row: 2.3 us.
 #include "common.h"
 #include "../../include/tgk_kernels.h"
 #include <cmath>
