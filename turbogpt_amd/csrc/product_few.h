@@ -177,7 +177,7 @@ template <class Kernel> void allow_lds(Kernel kernel, std::atomic<uint64_t> &con
 template <class T, class Epilogue> void launch_few(hipStream_t stream, Shape s, const Epilogue &epilogue) {
     s.tiles_m = (s.M + T::MT * 16 - 1) / (T::MT * 16), s.tiles_n = (s.N + T::NT * 16 - 1) / (T::NT * 16);
     s.stages = (s.k_bytes + STAGE - 1) / STAGE;
-    s.tiles = s.tiles_m * s.tiles_n; // at most 256, launch_product
+    s.tiles = s.tiles_m * s.tiles_n; // at most 256, product_kernel
     static std::atomic<uint64_t> configured;
     allow_lds(few_kernel<T, Epilogue>, configured, T::LDS_BYTES);
     hipLaunchKernelGGL((few_kernel<T, Epilogue>), dim3(s.tiles), dim3(FEW_WAVES * 64), T::LDS_BYTES, stream, s, epilogue);
